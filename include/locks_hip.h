@@ -41,7 +41,8 @@
 
 #include <stdint.h>
 
-#define LOCKS_ABI_VERSION 10
+#define LOCKS_ABI_VERSION 11
+#define LOCKS_TABLES_MAX_REQS 2048
 
 #ifdef __cplusplus
 extern "C" {
@@ -640,6 +641,74 @@ int32_t locks_mla_decode_dense(const uint16_t* q, int64_t q_stride_req, int64_t 
                                int64_t lse_stride_req, int32_t n_req, int32_t n_heads,
                                int32_t kv_lora_rank, int32_t rope_dim, int32_t page,
                                int32_t split, float scale, void* stream);
+
+/*
+ * Block tables, lengths, positions and cache slots of a step, from the
+ * requests' lengths.  The pool: table (max_reqs, table_stride) page ids and
+ * lens (max_reqs,) tokens of every row; free_list (num_blocks,), whose entries
+ * [head, num_blocks) are free, the next one first; state (4,) i32: head, the
+ * unserved requests of the last step, an arrival count (0 between calls).
+ * Batch entry r is row rows[r] (-1: padding) with new_lens[r] new tokens;
+ * it takes ceil((lens + new) / page) - ceil(lens / page) blocks, in batch
+ * order.  A request is served when they are there, its pages are at most
+ * max_pages, and its row exists and is named for the first time; else it
+ * changes nothing, its seq_len is 0 and its slots are -1.
+ *   block_table (n_req, bt_stride): the pages of each served request; other
+ *               entries stay as they were
+ *   seq_lens (n_req,), query_start_loc (n_req + 1,) i32
+ *   positions (n_tokens,) i32, slot_mapping (n_tokens,) i64: block * page +
+ *               offset; past the last request's tokens 0 and -1
+ * Rows of both tables hold a multiple of 4 ids, 16-byte aligned.  max_reqs <=
+ * LOCKS_TABLES_MAX_REQS, num_blocks <= 2^22.  Calls on one pool must not overlap.
+ */
+int32_t locks_tables_step(const int32_t* rows, const int32_t* new_lens, int32_t n_req,
+                          int32_t n_tokens, int32_t* lens, int32_t* table, int64_t table_stride,
+                          int32_t max_reqs, int32_t max_pages, const int32_t* free_list,
+                          int32_t num_blocks, int32_t* state, int32_t* block_table,
+                          int64_t bt_stride, int32_t* seq_lens, int32_t* query_start_loc,
+                          int32_t* positions, int64_t* slot_mapping, int32_t page, void* stream);
+
+/* Rows rows[r] back to min(lens, keep_lens[r]) tokens (a row named twice: the
+ * first): the blocks past them go in front of the free list, in the order in
+ * which a step takes blocks. */
+int32_t locks_tables_trim(const int32_t* rows, const int32_t* keep_lens, int32_t n_req,
+                          int32_t* lens, const int32_t* table, int64_t table_stride,
+                          int32_t max_reqs, int32_t max_pages, int32_t* free_list,
+                          int32_t num_blocks, int32_t* state, int32_t page, void* stream);
+
+/*
+ * Per token: RMS norm of each query and key head, rotation of its first `rot`
+ * entries, and the write of K and V into the paged cache.
+ *   q (n_tokens, n_heads, d), k, v (n_tokens, n_kv, d) bf16, element strides of
+ *   (token, head), d contiguous (views of one packed projection are fine)
+ *   y = x * rsqrt(mean(x^2) + eps) * weight   (a NULL weight: no norm for it;
+ *       weights (d,) bf16, or f32 with weights_f32)
+ *   pair (i, i + rot / 2), or with interleaved (2 i, 2 i + 1), of the first rot
+ *       entries: (a, b) -> (a cos_i - b sin_i, b cos_i + a sin_i) with
+ *       cos_sin[position] = rot / 2 cosines, then rot / 2 sines (f32, contiguous)
+ *   q_out (n_tokens, n_heads, d) bf16; may be q itself
+ *   k_out (n_tokens, n_kv, d) bf16 or NULL: the key rows as cached
+ *   k_cache / v_cache: block, token and kv head strides; slot = block * page +
+ *       offset.  A token whose slot is outside [0, num_blocks * page) writes no
+ *       cache row.  One whose position is outside [0, max_pos) writes none
+ *       either, and its q_out and k_out rows are NaN.  Tokens of one call have
+ *       distinct slots.
+ * All sums and products in fp32, one rounding to bf16.  rot a multiple of 16
+ * (0: no rotation), <= d in {64, 128, 256}; strides multiples of 8 elements,
+ * pointers 16-byte aligned.
+ */
+int32_t locks_qkv_write(const uint16_t* q, int64_t q_stride_tok, int64_t q_stride_head,
+                        const uint16_t* k, int64_t k_stride_tok, int64_t k_stride_head,
+                        const uint16_t* v, int64_t v_stride_tok, int64_t v_stride_head,
+                        const int32_t* positions, const int64_t* slot_mapping, uint16_t* k_cache,
+                        int64_t kc_stride_block, int64_t kc_stride_tok, int64_t kc_stride_head,
+                        uint16_t* v_cache, int64_t vc_stride_block, int64_t vc_stride_tok,
+                        int64_t vc_stride_head, int32_t num_blocks, const float* cos_sin,
+                        int32_t max_pos, int32_t rot, int32_t interleaved, const void* q_weight,
+                        const void* k_weight, int32_t weights_f32, float eps, uint16_t* q_out,
+                        int64_t qo_stride_tok, int64_t qo_stride_head, uint16_t* k_out,
+                        int64_t ko_stride_tok, int64_t ko_stride_head, int32_t n_tokens,
+                        int32_t n_heads, int32_t n_kv, int32_t head_dim, int32_t page, void* stream);
 
 #ifdef __cplusplus
 }

@@ -6,11 +6,12 @@ library.  If the library is missing the import of any hot-path entry raises
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 
 _LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_lib", "liblocks_hip.so")
-ABI_VERSION = 10
+ABI_VERSION = 11
 
 _c = ctypes
 _i32, _i64, _f32, _f64, _p = _c.c_int32, _c.c_int64, _c.c_float, _c.c_double, _c.c_void_p
@@ -93,6 +94,12 @@ SIGNATURES = {
     "locks_decode_dense": (_i32, [_p, _i64, _i64, _p, _i64, _i64, _i64, _p, _i64, _i64, _i64,
                                   _i32, _p, _i64, _i32, _p, _p, _p, _p, _p, _i64, _i64, _i32,
                                   _i32, _i32, _i32, _i32, _i32, _i32, _f32, _p]),
+    "locks_tables_step": (_i32, [_p, _p, _i32, _i32, _p, _p, _i64, _i32, _i32, _p, _i32, _p, _p,
+                                 _i64, _p, _p, _p, _p, _i32, _p]),
+    "locks_tables_trim": (_i32, [_p, _p, _i32, _p, _p, _i64, _i32, _i32, _p, _i32, _p, _i32, _p]),
+    "locks_qkv_write": (_i32, [_p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _p, _p, _p, _i64, _i64,
+                               _i64, _p, _i64, _i64, _i64, _i32, _p, _i32, _i32, _i32, _p, _p, _i32,
+                               _f32, _p, _i64, _i64, _p, _i64, _i64, _i32, _i32, _i32, _i32, _i32, _p]),
     "locks_decode_merge": (_i32, [_p, _p, _p, _p, _i64, _i32, _p, _i64, _i64, _i32, _i32, _i32,
                                   _i32, _i32, _i32, _i32, _i32, _p]),
 }
@@ -146,6 +153,16 @@ def rows_arg(st) -> int:
     row strides (a state with packed rows), or NULL (contiguous slabs)."""
     rb = getattr(st, "slab_row_bytes", None)
     return 0 if rb is None else _c.addressof(rb)
+
+
+_SAME = contextlib.nullcontext()
+
+
+def on_device(device):
+    """A context in which `device` (a torch.device with an index) is the current
+    one: a launch goes to the device of its tensors, whichever is current."""
+    import torch
+    return _SAME if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def stream_ptr(device=None) -> int:
