@@ -710,6 +710,79 @@ int32_t locks_qkv_write(const uint16_t* q, int64_t q_stride_tok, int64_t q_strid
                         int64_t ko_stride_tok, int64_t ko_stride_head, int32_t n_tokens,
                         int32_t n_heads, int32_t n_kv, int32_t head_dim, int32_t page, void* stream);
 
+/*
+ * Attention over the paged cache.  Common to the three entries below:
+ *   q, out (rows, n_kv * G, head_dim) bf16, element strides of (row, head);
+ *   lse (rows, n_kv * G) f32 with row stride, or NULL: natural log of the sum
+ *   of exp(scale * q.k) over the visible keys; K / V as for locks_decode_splitk
+ *   block_table (n_req, bt_cols) i32: block ids are clamped to [0, num_blocks)
+ *   seq_lens (n_req,) i32, this step's tokens included; a length past bt_cols *
+ *   page sees only the table's tokens
+ *   A row that sees no key (seq_len 0: padding) is 0, its lse -inf.  What lies
+ *   in masked places of the cache (unwritten pages, tokens out of the window or
+ *   after the query), NaN and infinities included, does not matter.
+ *   scale > 0.  fp32 scores, softmax and sums; the weights are rounded to bf16
+ *   for the product with V.
+ *   max_seq_len  host-side upper bound of seq_lens (0: the table's width); only
+ *                sizes the launch
+ *   workspace    16-byte aligned device memory, workspace_bytes >= what the call
+ *                needs: locks_attn_workspace_bytes(max_tokens, ...) covers single-
+ *                token calls of up to max_tokens requests (in up to max_tokens
+ *                groups) and every locks_window_prefill call of up to max_tokens
+ *                tokens.  Its content is undefined between calls; calls that
+ *                share one must not overlap.
+ */
+int64_t locks_attn_workspace_bytes(int32_t max_tokens, int32_t n_kv, int32_t G, int32_t head_dim);
+
+/* One query per request at position seq_len - 1: keys [max(seq_len - window, 0),
+ * seq_len) and [0, sinks); window 0: all keys. */
+int32_t locks_window_decode(const uint16_t* q, int64_t q_stride_req, int64_t q_stride_head,
+                            const uint16_t* k_cache, int64_t k_stride_block, int64_t k_stride_tok,
+                            int64_t k_stride_head, const uint16_t* v_cache, int64_t v_stride_block,
+                            int64_t v_stride_tok, int64_t v_stride_head, int32_t num_blocks,
+                            const int32_t* block_table, int64_t bt_stride, int32_t bt_cols,
+                            const int32_t* seq_lens, int32_t window, int32_t sinks, uint16_t* out,
+                            int64_t out_stride_req, int64_t out_stride_head, float* lse,
+                            int64_t lse_stride_req, void* workspace, int64_t workspace_bytes,
+                            int32_t n_req, int32_t n_kv, int32_t G, int32_t head_dim, int32_t page,
+                            int32_t max_seq_len, float scale, void* stream);
+
+/* Many queries per request: rows [query_start_loc[r], query_start_loc[r + 1]) of
+ * q, the last one at position seq_len - 1.  The query at position p sees keys
+ * [max(p - window + 1, 0), p] and [0, min(sinks, p + 1)); window 0: [0, p].
+ * Rows from query_start_loc[n_req] on stay as they were; n_tokens bounds them. */
+int32_t locks_window_prefill(const uint16_t* q, int64_t q_stride_tok, int64_t q_stride_head,
+                             const uint16_t* k_cache, int64_t k_stride_block, int64_t k_stride_tok,
+                             int64_t k_stride_head, const uint16_t* v_cache, int64_t v_stride_block,
+                             int64_t v_stride_tok, int64_t v_stride_head, int32_t num_blocks,
+                             const int32_t* block_table, int64_t bt_stride, int32_t bt_cols,
+                             const int32_t* seq_lens, const int32_t* query_start_loc, int32_t window,
+                             int32_t sinks, uint16_t* out, int64_t out_stride_tok,
+                             int64_t out_stride_head, float* lse, int64_t lse_stride_tok,
+                             void* workspace, int64_t workspace_bytes, int32_t n_tokens,
+                             int32_t n_req, int32_t n_kv, int32_t G, int32_t head_dim, int32_t page,
+                             int32_t max_seq_len, float scale, void* stream);
+
+/* One query per request over all its keys, where the requests [group_start[g],
+ * group_start[g + 1]) (group_start (n_groups + 1,) ascending) share their first
+ * prefix_pages[g] pages: these are read once for the group, through the block
+ * table row of its first request.  A member shorter than the prefix sees only its
+ * own length.  A request in no group is attended like any other.
+ *   max_prefix_pages  host-side upper bound of prefix_pages (0: none); only sizes
+ *                     the launch */
+int32_t locks_prefix_decode(const uint16_t* q, int64_t q_stride_req, int64_t q_stride_head,
+                            const uint16_t* k_cache, int64_t k_stride_block, int64_t k_stride_tok,
+                            int64_t k_stride_head, const uint16_t* v_cache, int64_t v_stride_block,
+                            int64_t v_stride_tok, int64_t v_stride_head, int32_t num_blocks,
+                            const int32_t* block_table, int64_t bt_stride, int32_t bt_cols,
+                            const int32_t* seq_lens, const int32_t* group_start,
+                            const int32_t* prefix_pages, int32_t n_groups, uint16_t* out,
+                            int64_t out_stride_req, int64_t out_stride_head, float* lse,
+                            int64_t lse_stride_req, void* workspace, int64_t workspace_bytes,
+                            int32_t n_req, int32_t n_kv, int32_t G, int32_t head_dim, int32_t page,
+                            int32_t max_prefix_pages, int32_t max_seq_len, float scale,
+                            void* stream);
+
 #ifdef __cplusplus
 }
 #endif

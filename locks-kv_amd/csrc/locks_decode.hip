@@ -25,11 +25,13 @@
 //     transpose: the output d-index of MFMA block `blk`, row i is 8*i + blk,
 //     so each lane's four 16-byte V row loads ARE its A operand.  The softmax
 //     rescale is a per-lane scalar because O^T keeps one head per lane.
+#include "locks_attn.h"
 #include "locks_common.h"
 #include "locks_hip.h"
 
 #include <algorithm>
 #include <mutex>
+#include <type_traits>
 
 namespace locks {
 
@@ -39,6 +41,8 @@ constexpr int DC_BLK = DC_WAVES * kWave;
 typedef __attribute__((address_space(3))) void* lds_ptr;
 typedef __attribute__((address_space(3))) const uint8_t* lds_u8_ptr;
 typedef int v2i __attribute__((ext_vector_type(2)));
+typedef short v4s __attribute__((ext_vector_type(4)));
+typedef __bf16 v4bf __attribute__((ext_vector_type(4)));
 constexpr int MAX_SPLIT = 512;
 constexpr int DENSE_NST = 2;           // page stages per wave of the dense comparator
 // K/V DMA cache policy: NT (non-temporal: every page is read once) measured
@@ -271,7 +275,11 @@ struct TierSrc {
     int lidx, k_tier;
 };
 
-template <bool FUSED, bool DENSE = false, int NST = 2, int KVPOL = 0, int D = 128, bool TIER = false>
+// RANGE (with DENSE's contiguous steps): the tokens of RangeSrc, split by
+// 16-token steps instead of pages.  P stays bf16 like V, so that V's whole range
+// holds, and V rows that the range leaves out count as zero, whatever they hold.
+template <bool FUSED, bool DENSE = false, int NST = 2, int KVPOL = 0, int D = 128, bool TIER = false,
+          bool RANGE = false>
 __global__ __launch_bounds__(DC_BLK) void decode_split_kernel(
     const uint16_t* __restrict__ q, long q_sr, long q_sh,
     const uint16_t* __restrict__ kc, long k_sb, long k_st, long k_sh,
@@ -282,10 +290,11 @@ __global__ __launch_bounds__(DC_BLK) void decode_split_kernel(
     float* __restrict__ m_part, float* __restrict__ l_part, float* __restrict__ acc_part,
     int G, int split, int pps_min, float sm_scale, int pg_sh,
     int* __restrict__ counters, void* __restrict__ out, long o_sr, long o_sh, int out_f32,
-    const TierSrc tier)
+    const std::conditional_t<RANGE, RangeSrc, TierSrc> tier)
 {
     using GM = DcGeom<D>;
     static_assert(!(TIER && (FUSED || DENSE)), "the tier source serves the split kernel");
+    static_assert(!RANGE || (DENSE && !FUSED), "a range is a part of the dense rows");
     constexpr int KS = GM::KS, DPL = GM::DPL, NI = GM::NI, KB = GM::KBYTES, SB = GM::STEP_BYTES;
     const int sp = blockIdx.x, kh = blockIdx.y, r = blockIdx.z;
     const int n_kv = gridDim.y;
@@ -299,7 +308,20 @@ __global__ __launch_bounds__(DC_BLK) void decode_split_kernel(
     // case), loaded together with the page count instead of after it.
     const int js = ((sp * pps_min) << pg_sh) + wave + DC_WAVES * lane;
     int pt_spec = 0, cnt;
-    if constexpr (DENSE) {
+    int lo = 0, sinks = 0, n_sink = 0, t_gap = 0;       // RANGE: first key, first keys; steps of those, steps skipped
+    if constexpr (RANGE) {
+        const int n = (int)min((long)seq_lens[r], (long)bt_cols * PG);
+        if (tier.n_groups) {
+            const int g = group_of(tier.gstart, tier.n_groups, r);
+            lo = g < 0 ? 0 : (int)min((long)max(tier.gpages[g], 0) * PG, (long)max(n, 0));
+        } else {
+            lo = tier.window ? max(n - tier.window, 0) : 0;
+        }
+        sinks = min(tier.sinks, lo);
+        n_sink = (sinks + DC_PG - 1) / DC_PG;
+        t_gap = max(lo / DC_PG - n_sink, 0);
+        cnt = n > 0 ? (n + DC_PG - 1) / DC_PG - t_gap : 0;
+    } else if constexpr (DENSE) {
         cnt = min(cdiv(seq_lens[r], PG), bt_cols);
     } else {
         pt_spec = ((js >> pg_sh) < pt_cols) ? prow[js >> pg_sh] : 0;
@@ -307,6 +329,14 @@ __global__ __launch_bounds__(DC_BLK) void decode_split_kernel(
     }
     // gridDim.x = the launched split count (<= split, the buffers' stride)
     const int nsplit = gridDim.x;
+    if constexpr (RANGE) {
+        // a request in no group has no partials of a prefix
+        if (tier.n_groups && sp == 0 && group_of(tier.gstart, tier.n_groups, r) < 0)
+            for (int i = tid; i < tier.first_split * G; i += DC_BLK) {
+                m_part[rk * split * G + i] = -INFINITY;
+                l_part[rk * split * G + i] = 0.f;
+            }
+    }
     const int pps = max(cdiv(cnt, nsplit), pps_min);
     const int j0 = sp * pps;
     if constexpr (FUSED) {
@@ -320,12 +350,20 @@ __global__ __launch_bounds__(DC_BLK) void decode_split_kernel(
             return;
         }
     }
+    if constexpr (RANGE) {
+        if (j0 >= cnt) {
+            const long i = (rk * split + tier.first_split + sp) * G + tid;
+            if (tid < G) { m_part[i] = -INFINITY; l_part[i] = 0.f; }
+            return;
+        }
+    }
     if (j0 >= cnt) return;                        // inactive split: no store
     const int j1 = min(j0 + pps, cnt);
-    const int s0 = j0 << pg_sh, s1 = j1 << pg_sh; // this split's 16-token steps
+    // this split's 16-token steps
+    const int s0 = RANGE ? j0 : j0 << pg_sh, s1 = RANGE ? j1 : j1 << pg_sh;
 
     const int c16 = lane & 15, kg = lane >> 4;
-    const int seq_len = seq_lens[r];
+    const int seq_len = RANGE ? (int)min((long)seq_lens[r], (long)bt_cols * PG) : seq_lens[r];
 
     // NST step stages per wave (stage 0 in stA, the others in stB), later
     // reused for the merges (the fused merge needs MAX_SPLIT x 16 floats in each)
@@ -361,9 +399,10 @@ __global__ __launch_bounds__(DC_BLK) void decode_split_kernel(
         ptv = 0;
         blkv = 0;
         if (jj < s1) {
-            if constexpr (DENSE) ptv = jj >> pg_sh;
+            if constexpr (RANGE) ptv = jj + (jj >= n_sink ? t_gap : 0);    // the 16-token step of the row
+            else if constexpr (DENSE) ptv = jj >> pg_sh;
             else ptv = spec ? pt_spec : prow[jj >> pg_sh];
-            const int ptc = min(max(ptv, 0), bt_cols - 1);
+            const int ptc = min(max(RANGE ? ptv >> pg_sh : ptv, 0), bt_cols - 1);
             blkv = min(max(bt[(long)r * bt_sr + ptc], 0), NB - 1);
             if constexpr (TIER) {                 // the tier's keys of (kv head, block)
                 slotv = tier.p2s[(long)kh * NB + blkv];
@@ -377,7 +416,7 @@ __global__ __launch_bounds__(DC_BLK) void decode_split_kernel(
     //   V (D >= 128) slot (i, hh) = V[4 kg + i][DPL (lane&15) + 8 hh ..];
     //   V (D == 64) in natural row order (8 lanes per 128-byte row).
     auto issue = [&](int s, int sub, uint8_t* st) -> int {
-        const int pt = __builtin_amdgcn_readlane(ptv, s);
+        [[maybe_unused]] const int pt = __builtin_amdgcn_readlane(ptv, s);
         const int blk = __builtin_amdgcn_readlane(blkv, s);
         const long t0 = (long)sub * 16;
         const uint16_t* kpage = kc + (long)blk * k_sb + (long)kh * k_sh;
@@ -432,7 +471,9 @@ __global__ __launch_bounds__(DC_BLK) void decode_split_kernel(
         // tell these reads from the other stages' DMA still in flight and
         // would otherwise wait for every outstanding load (vmcnt(0)) here.
         // The caller has already waited for this stage's own DMA.  One asm
-        // block per head_dim, so nothing uses a result before the wait.
+        // block per head_dim, so nothing uses a result before the wait; outputs
+        // are early-clobber: the first reads write theirs while the last ones
+        // still take the address.
         v4i kr[KS];
         uint32_t vw[4][DPL / 2];                     // V row v: DPL bf16 columns
         const uint32_t sbase = (uint32_t)(uintptr_t)(lds_u8_ptr)(st);
@@ -448,7 +489,7 @@ __global__ __launch_bounds__(DC_BLK) void decode_split_kernel(
                 "ds_read_b64 %4, %7 offset:256\n\t"
                 "ds_read_b64 %5, %7 offset:384\n\t"
                 "s_waitcnt lgkmcnt(0)"
-                : "=v"(kr[0]), "=v"(kr[1]), "=v"(v64[0]), "=v"(v64[1]), "=v"(v64[2]), "=v"(v64[3])
+                : "=&v"(kr[0]), "=&v"(kr[1]), "=&v"(v64[0]), "=&v"(v64[1]), "=&v"(v64[2]), "=&v"(v64[3])
                 : "v"(la), "v"(lv));
 #pragma unroll
             for (int v = 0; v < 4; ++v) { vw[v][0] = (uint32_t)v64[v][0]; vw[v][1] = (uint32_t)v64[v][1]; }
@@ -464,8 +505,8 @@ __global__ __launch_bounds__(DC_BLK) void decode_split_kernel(
                 "ds_read_b128 %6, %8 offset:6144\n\t"
                 "ds_read_b128 %7, %8 offset:7168\n\t"
                 "s_waitcnt lgkmcnt(0)"
-                : "=v"(kr[0]), "=v"(kr[1]), "=v"(kr[2]), "=v"(kr[3]),
-                  "=v"(vr[0]), "=v"(vr[1]), "=v"(vr[2]), "=v"(vr[3])
+                : "=&v"(kr[0]), "=&v"(kr[1]), "=&v"(kr[2]), "=&v"(kr[3]),
+                  "=&v"(vr[0]), "=&v"(vr[1]), "=&v"(vr[2]), "=&v"(vr[3])
                 : "v"(la));
 #pragma unroll
             for (int v = 0; v < 4; ++v)
@@ -492,10 +533,10 @@ __global__ __launch_bounds__(DC_BLK) void decode_split_kernel(
                 "ds_read_b128 %14, %17 offset:6144\n\t"
                 "ds_read_b128 %15, %17 offset:7168\n\t"
                 "s_waitcnt lgkmcnt(0)"
-                : "=v"(kr[0]), "=v"(kr[1]), "=v"(kr[2]), "=v"(kr[3]),
-                  "=v"(kr[4]), "=v"(kr[5]), "=v"(kr[6]), "=v"(kr[7]),
-                  "=v"(vr[0]), "=v"(vr[1]), "=v"(vr[2]), "=v"(vr[3]),
-                  "=v"(vr[4]), "=v"(vr[5]), "=v"(vr[6]), "=v"(vr[7])
+                : "=&v"(kr[0]), "=&v"(kr[1]), "=&v"(kr[2]), "=&v"(kr[3]),
+                  "=&v"(kr[4]), "=&v"(kr[5]), "=&v"(kr[6]), "=&v"(kr[7]),
+                  "=&v"(vr[0]), "=&v"(vr[1]), "=&v"(vr[2]), "=&v"(vr[3]),
+                  "=&v"(vr[4]), "=&v"(vr[5]), "=&v"(vr[6]), "=&v"(vr[7])
                 : "v"(la), "v"(la2));
             // slot (v, hh) = vr[2 v + hh]: columns 16 c16 + 8 hh ..
 #pragma unroll
@@ -508,10 +549,25 @@ __global__ __launch_bounds__(DC_BLK) void decode_split_kernel(
 #pragma unroll
         for (int i = 0; i < KS; ++i)
             s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, kr[i]), qb[i], s, 0, 0, 0);
-        const int pos0 = pt * PG + sub * 16 + 4 * kg;
+        const int pos0 = RANGE ? pt * 16 + 4 * kg : pt * PG + sub * 16 + 4 * kg;
         float sv[4];
 #pragma unroll
         for (int v = 0; v < 4; ++v) sv[v] = (pos0 + v < seq_len) ? s[v] * sm_scale : -INFINITY;
+        if constexpr (RANGE) {
+            // a step that the range cuts: keys before lo that are none of the
+            // first, keys past the row (a step is one or the other, or both)
+            const int t0 = pt * 16;
+            if (t0 + 16 > seq_len || (t0 < lo && t0 + 16 > sinks)) {
+#pragma unroll
+                for (int v = 0; v < 4; ++v) {
+                    const int p = pos0 + v;
+                    const bool seen = p < seq_len && (p >= lo || p < sinks);
+                    sv[v] = seen ? sv[v] : -INFINITY;
+#pragma unroll
+                    for (int e = 0; e < DPL / 2; ++e) vw[v][e] = seen ? vw[v][e] : 0u;
+                }
+            }
+        }
         // ---- online softmax (head = lane column) ------------------------
         float mx = fmaxf(fmaxf(sv[0], sv[1]), fmaxf(sv[2], sv[3]));
         mx = xor32_max(xor16_max(mx));
@@ -523,6 +579,19 @@ __global__ __launch_bounds__(DC_BLK) void decode_split_kernel(
         for (int v = 0; v < 4; ++v) p[v] = __expf(sv[v] - m_ref);
         lsum = lsum * alpha + (p[0] + p[1] + p[2] + p[3]);
         m = m_new;
+        if constexpr (RANGE) {
+            const v4bf pr = {(__bf16)p[0], (__bf16)p[1], (__bf16)p[2], (__bf16)p[3]};
+            const v4s pb = __builtin_bit_cast(v4s, pr);
+#pragma unroll
+            for (int b = 0; b < DPL; ++b) {
+                const uint32_t sel = (b & 1) ? 0x07060302u : 0x05040100u;
+                const v2i a = {(int)__builtin_amdgcn_perm(vw[1][b >> 1], vw[0][b >> 1], sel),
+                               (int)__builtin_amdgcn_perm(vw[3][b >> 1], vw[2][b >> 1], sel)};
+                o[b] = o[b] * alpha;
+                o[b] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(v4s, a), pb, o[b], 0, 0, 0);
+            }
+            return;
+        }
         const v4h pb = {(_Float16)p[0], (_Float16)p[1], (_Float16)p[2], (_Float16)p[3]};
         // ---- O^T[d][g] += V^T P^T: block b holds d = DPL * row + b --------
 #pragma unroll
@@ -542,7 +611,9 @@ __global__ __launch_bounds__(DC_BLK) void decode_split_kernel(
         fetch_ids(jb, pps == pps_min && jb == s0 + wave);
         __builtin_amdgcn_s_waitcnt(0x0070);   // ids (and q) resident before any DMA
         const int ns = min(kWave, cdiv(s1 - jb, DC_WAVES));   // steps of this batch
-        auto sub_of = [&](int s) { return (jb + DC_WAVES * s) & smask; };
+        auto sub_of = [&](int s) {
+            return (RANGE ? __builtin_amdgcn_readlane(ptv, s) : jb + DC_WAVES * s) & smask;
+        };
         // ring of NST stages: step s + NST - 1 is issued before step s is
         // consumed, so up to NST - 1 steps stream while one is scored
 #pragma unroll
@@ -576,7 +647,8 @@ __global__ __launch_bounds__(DC_BLK) void decode_split_kernel(
                     make_float4(o[4 * j][v], o[4 * j + 1][v], o[4 * j + 2][v], o[4 * j + 3][v]);
     }
     __syncthreads();
-    const long base = (rk * split + sp) * G;
+    long base = (rk * split + sp) * G;
+    if constexpr (RANGE) base += (long)tier.first_split * G;
     for (int i = tid; i < G * (D / 4); i += DC_BLK) {
         const int g = i / (D / 4), d = (i % (D / 4)) * 4;
         float M = wm[0][g];
@@ -1068,6 +1140,22 @@ extern "C" int32_t locks_decode_merge(
     return check_launch("decode_merge_kernel");
 }
 
+
+namespace locks {
+int launch_decode_range(const uint16_t* q, long q_sr, long q_sh, const uint16_t* k, const long* ks, const uint16_t* v,
+                        const long* vs, int num_blocks, const int* bt, long bt_sr, int bt_cols, const int* seq_lens,
+                        const Partials& p, const RangeSrc& range, int nsplit, int min_steps, int n_req, int n_kv, int G,
+                        int head_dim, int page, float scale, hipStream_t stream) {
+    const int pg_sh = page == 16 ? 0 : page == 32 ? 1 : 2;
+#define LAUNCH_D(DV)                                                                                                  hipLaunchKernelGGL((decode_split_kernel<false, true, DENSE_NST, CPOL_NT, DV, false, true>),                                          dim3(nsplit, n_kv, n_req), dim3(DC_BLK), 0, stream, q, q_sr, q_sh, k, ks[0], ks[1], ks[2], \
+                       v, vs[0], vs[1], vs[2], num_blocks, bt, bt_sr, bt_cols, nullptr, 0L, 0L, 1, nullptr, 0L,   \
+                       seq_lens, p.m, p.l, p.acc, G, p.splits, min_steps, scale, pg_sh, nullptr, nullptr, 0L, 0L, \
+                       0, range)
+    DC_BY_D(head_dim, LAUNCH_D);
+#undef LAUNCH_D
+    return check_launch("decode_split_kernel<range>");
+}
+}  // namespace locks
 
 extern "C" int32_t locks_decode_dense(
     const uint16_t* q, int64_t q_stride_req, int64_t q_stride_head,

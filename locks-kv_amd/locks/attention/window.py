@@ -1,0 +1,130 @@
+"""Attention over the whole paged cache or a sliding window of it.
+
+The dense layers that stand between the selected ones: ``window_decode`` (one
+new token per request) and ``window_prefill`` (prompt chunks, mixed batches)
+attend to the last ``window`` tokens and to the first ``sinks`` ones, or to
+everything; ``prefix_decode`` reads the pages that a group of requests shares
+once for the whole group.
+"""
+from __future__ import annotations
+
+import torch
+
+from .. import _lib
+from .decode import _kv_args
+
+
+def attn_workspace(device, *, max_tokens: int, n_kv: int, G: int, head_dim: int) -> torch.Tensor:
+    """Workspace of the calls in this module, allocated once: single-token calls
+    of up to ``max_tokens`` requests and prefill calls of up to ``max_tokens``
+    tokens.  Calls that share it follow each other."""
+    if max_tokens < 1 or n_kv < 1 or not 1 <= G <= 16 or head_dim not in (64, 128, 256):
+        raise ValueError(f"max_tokens {max_tokens}, n_kv {n_kv}, G {G}, head_dim {head_dim}: need positive counts, "
+                         "G in [1, 16], head_dim 64, 128 or 256")
+    n = _lib.load().locks_attn_workspace_bytes(int(max_tokens), int(n_kv), int(G), int(head_dim))
+    return torch.empty(n, dtype=torch.uint8, device=device)
+
+
+def _i32(name: str, t, n: int, device) -> None:
+    if t.dtype != torch.int32 or t.dim() != 1 or (t.numel() > 1 and t.stride(0) != 1):
+        raise TypeError(f"{name} must be a contiguous int32 vector, got {t.dtype} {tuple(t.shape)}")
+    if t.shape[0] < n or t.device != device:
+        raise ValueError(f"{name} must hold {n} entries on {device}, got {t.shape[0]} on {t.device}")
+
+
+def _args(what: str, q, kv_cache, block_table, seq_lens, out, ws, lse, rows: int, n_req: int):
+    """The checks that the calls share, and their common arguments: (head, of q
+    up to seq_lens; tail, from out to the workspace; n_kv, G, d, page; device)."""
+    if kv_cache.dim() != 5 or kv_cache.dtype != torch.bfloat16 or kv_cache.stride(-1) != 1:
+        raise TypeError(f"{what}: kv_cache must be a 5-d bf16 cache with a contiguous last dim, got "
+                        f"{kv_cache.dtype} {tuple(kv_cache.shape)}")
+    kp, vp, ks, (NB, page, n_kv, d) = _kv_args(kv_cache)
+    if vp is None:
+        raise ValueError(f"{what} needs a cache with a V half")
+    dev = kv_cache.device
+    for name, t in (("q", q), ("out", out)):
+        if t.dtype != torch.bfloat16 or t.dim() != 3 or t.stride(-1) != 1:
+            raise TypeError(f"{what}: {name} must be bf16 (rows, heads, d) with a contiguous last dim, got {t.dtype} "
+                            f"{tuple(t.shape)} strides {t.stride()}")
+        if t.shape[0] < rows or t.shape[2] != d or t.shape[1] % n_kv or t.shape[1] != q.shape[1]:
+            raise ValueError(f"{what}: {name} has shape {tuple(t.shape)}; the call has {rows} rows, head_dim {d} and a "
+                             f"multiple of {n_kv} heads")
+        if t.device != dev:
+            raise ValueError(f"{what}: {name} is on {t.device}, the cache on {dev}")
+    H = int(q.shape[1])
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.stride(1) != 1:
+        raise TypeError(f"{what}: block_table must be int32 (requests, pages) with contiguous rows")
+    if block_table.shape[0] < n_req or block_table.device != dev:
+        raise ValueError(f"{what}: block_table must hold {n_req} rows on {dev}, got {block_table.shape[0]} on "
+                         f"{block_table.device}")
+    _i32(f"{what}: seq_lens", seq_lens, n_req, dev)
+    ls = 0
+    if lse is not None:
+        if lse.dtype != torch.float32 or lse.dim() != 2 or lse.stride(1) != 1:
+            raise TypeError(f"{what}: lse must be fp32 (rows, heads) with contiguous rows")
+        if lse.shape[0] < rows or lse.shape[1] != H or lse.device != dev:
+            raise ValueError(f"{what}: lse must be ({rows}, {H}) on {dev}, got {tuple(lse.shape)} on {lse.device}")
+        ls = lse.stride(0)
+    if ws is not None and (ws.device != dev or not ws.is_contiguous()):
+        raise ValueError(f"{what}: the workspace must be contiguous, on {dev}")
+    if dev.type != "cuda":
+        raise ValueError(f"{what} runs on the GPU, the cache is on {dev}")
+    head = (q.data_ptr(), *q.stride()[:2], kp, *ks, vp, *ks, NB, block_table.data_ptr(), block_table.stride(0),
+            int(block_table.shape[1]), seq_lens.data_ptr())
+    tail = (out.data_ptr(), *out.stride()[:2], _lib.ptr(lse), ls, _lib.ptr(ws),
+            0 if ws is None else ws.numel() * ws.element_size())
+    return head, tail, (n_kv, H // n_kv, d, page), dev
+
+
+def window_decode(q, kv_cache, block_table, seq_lens, out, ws, *, n_req: int, scale: float, window: int = 0,
+                  sinks: int = 0, lse=None, max_seq_len: int = 0) -> None:
+    """One new token per request, at position ``seq_lens - 1``: ``out[:n_req]``
+    (T, H, d) bf16 = softmax attention of ``q`` over the keys of the last
+    ``window`` positions, its own included, and of the first ``sinks`` (window 0:
+    all), and ``lse[:n_req]`` (T, H) fp32 the log-sum-exp of the scores.  A request
+    of length 0 (padding) gives zeros and -inf.  ``max_seq_len``: an upper bound of
+    the lengths, where one is known, sizes the launch.  ``ws``: attn_workspace."""
+    head, tail, geo, dev = _args("window_decode", q, kv_cache, block_table, seq_lens, out, ws, lse, n_req, n_req)
+    if n_req == 0:
+        return
+    with _lib.on_device(dev):
+        _lib.check(_lib.load().locks_window_decode(*head, int(window), int(sinks), *tail, int(n_req), *geo,
+                                                   int(max_seq_len), float(scale), _lib.stream_ptr(dev)),
+                   "window_decode")
+
+
+def window_prefill(q, kv_cache, block_table, seq_lens, query_start_loc, out, ws, *, n_req: int, scale: float,
+                   window: int = 0, sinks: int = 0, lse=None, n_tokens: int = None, max_seq_len: int = 0) -> None:
+    """Rows ``query_start_loc[r] .. query_start_loc[r + 1]`` of ``q`` (T, H, d)
+    are the last tokens of request r, whose K and V are in the cache; each sees
+    the keys up to its own position, in the window or among the first ``sinks`` as
+    for ``window_decode``.  Rows from ``query_start_loc[n_req]`` on stay as they
+    were.  ``n_tokens`` (default: the rows of q) bounds the rows read."""
+    n_tokens = int(q.shape[0] if n_tokens is None else n_tokens)
+    head, tail, geo, dev = _args("window_prefill", q, kv_cache, block_table, seq_lens, out, ws, lse, n_tokens, n_req)
+    _i32("window_prefill: query_start_loc", query_start_loc, n_req + 1, dev)
+    if n_req == 0 or n_tokens == 0:
+        return
+    with _lib.on_device(dev):
+        _lib.check(_lib.load().locks_window_prefill(
+            *head, query_start_loc.data_ptr(), int(window), int(sinks), *tail, n_tokens, int(n_req), *geo,
+            int(max_seq_len), float(scale), _lib.stream_ptr(dev)), "window_prefill")
+
+
+def prefix_decode(q, kv_cache, block_table, seq_lens, group_start, prefix_pages, out, ws, *, n_req: int,
+                  n_groups: int, scale: float, lse=None, max_prefix_pages: int = 0, max_seq_len: int = 0) -> None:
+    """``window_decode`` without a window for requests that share pages: requests
+    ``group_start[g] .. group_start[g + 1]`` (ascending) hold the same ids in their
+    first ``prefix_pages[g]`` columns, which are read once for the group, through
+    the row of its first request.  Both are int32 on the GPU, so that a captured
+    call follows them.  Requests outside all groups, members shorter than the
+    prefix and padding (length 0) are attended like any other."""
+    head, tail, geo, dev = _args("prefix_decode", q, kv_cache, block_table, seq_lens, out, ws, lse, n_req, n_req)
+    _i32("prefix_decode: group_start", group_start, n_groups + 1, dev)
+    _i32("prefix_decode: prefix_pages", prefix_pages, n_groups, dev)
+    if n_req == 0:
+        return
+    with _lib.on_device(dev):
+        _lib.check(_lib.load().locks_prefix_decode(
+            *head, group_start.data_ptr(), prefix_pages.data_ptr(), int(n_groups), *tail, int(n_req), *geo,
+            int(max_prefix_pages), int(max_seq_len), float(scale), _lib.stream_ptr(dev)), "prefix_decode")
