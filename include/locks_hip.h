@@ -726,13 +726,13 @@ int32_t locks_qkv_write(const uint16_t* q, int64_t q_stride_tok, int64_t q_strid
  *   max_seq_len  host-side upper bound of seq_lens (0: the table's width); only
  *                sizes the launch
  *   workspace    16-byte aligned device memory, workspace_bytes >= what the call
- *                needs: locks_attn_workspace_bytes(max_tokens, ...) covers single-
- *                token calls of up to max_tokens requests (in up to max_tokens
- *                groups) and every locks_window_prefill call of up to max_tokens
- *                tokens.  Its content is undefined between calls; calls that
+ *                needs: locks_attn_workspace_bytes covers single-token calls of up
+ *                to max_reqs requests and locks_window_prefill calls of up to
+ *                max_tokens tokens.  Its content is undefined between calls; calls that
  *                share one must not overlap.
  */
-int64_t locks_attn_workspace_bytes(int32_t max_tokens, int32_t n_kv, int32_t G, int32_t head_dim);
+int64_t locks_attn_workspace_bytes(int32_t max_reqs, int32_t max_tokens, int32_t n_kv, int32_t G,
+                                   int32_t head_dim);
 
 /* One query per request at position seq_len - 1: keys [max(seq_len - window, 0),
  * seq_len) and [0, sinks); window 0: all keys. */

@@ -529,14 +529,15 @@ static long bound_keys(int32_t max_seq_len, int32_t bt_cols, int32_t page) {
     return max_seq_len > 0 && max_seq_len < cap ? max_seq_len : cap;
 }
 
-extern "C" int64_t locks_attn_workspace_bytes(int32_t max_tokens, int32_t n_kv, int32_t G, int32_t head_dim)
+extern "C" int64_t locks_attn_workspace_bytes(int32_t max_reqs, int32_t max_tokens, int32_t n_kv, int32_t G,
+                                              int32_t head_dim)
 {
-    if (max_tokens < 1 || n_kv < 1 || G < 1 || G > 16 || head_dim < 1) return 0;
+    if (max_reqs < 0 || max_tokens < 0 || n_kv < 1 || G < 1 || G > 16 || head_dim < 1) return 0;
     const long long_row = 0x7fffffc0L;
     int64_t most = 0;
-    // single-token calls of up to max_tokens requests, with and without a prefix
-    // (as many groups as requests at most); calls of many tokens in one request or more
-    for (int n = 1; n <= (max_tokens < 65535 ? max_tokens : 65535); ++n) {
+    // single-token calls of up to max_reqs requests, with a prefix (of one group:
+    // more of them make fewer splits); calls of many tokens, of one request (ditto)
+    for (int n = 1; n <= (max_reqs < 65535 ? max_reqs : 65535); ++n) {
         const int own = decode_splits(n, n_kv, long_row);
         const int shr = shared_splits(prefill_tiles(n, 1, G), n_kv, long_row, head_dim);
         const int64_t b = part_bytes((int64_t)n * n_kv * G, own + shr, head_dim);

@@ -100,7 +100,7 @@ SIGNATURES = {
     "locks_qkv_write": (_i32, [_p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _p, _p, _p, _i64, _i64,
                                _i64, _p, _i64, _i64, _i64, _i32, _p, _i32, _i32, _i32, _p, _p, _i32,
                                _f32, _p, _i64, _i64, _p, _i64, _i64, _i32, _i32, _i32, _i32, _i32, _p]),
-    "locks_attn_workspace_bytes": (_i64, [_i32, _i32, _i32, _i32]),
+    "locks_attn_workspace_bytes": (_i64, [_i32, _i32, _i32, _i32, _i32]),
     "locks_window_decode": (_i32, [_p, _i64, _i64, _p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _i32, _p,
                                    _i64, _i32, _p, _i32, _i32, _p, _i64, _i64, _p, _i64, _p, _i64, _i32,
                                    _i32, _i32, _i32, _i32, _i32, _f32, _p]),

@@ -14,14 +14,15 @@ from .. import _lib
 from .decode import _kv_args
 
 
-def attn_workspace(device, *, max_tokens: int, n_kv: int, G: int, head_dim: int) -> torch.Tensor:
+def attn_workspace(device, *, max_tokens: int, n_kv: int, G: int, head_dim: int, max_reqs: int = None) -> torch.Tensor:
     """Workspace of the calls in this module, allocated once: single-token calls
-    of up to ``max_tokens`` requests and prefill calls of up to ``max_tokens``
-    tokens.  Calls that share it follow each other."""
-    if max_tokens < 1 or n_kv < 1 or not 1 <= G <= 16 or head_dim not in (64, 128, 256):
-        raise ValueError(f"max_tokens {max_tokens}, n_kv {n_kv}, G {G}, head_dim {head_dim}: need positive counts, "
-                         "G in [1, 16], head_dim 64, 128 or 256")
-    n = _lib.load().locks_attn_workspace_bytes(int(max_tokens), int(n_kv), int(G), int(head_dim))
+    of up to ``max_reqs`` requests (default: ``max_tokens``) and prefill calls of up
+    to ``max_tokens`` tokens.  Calls that share it follow each other."""
+    max_reqs = max_tokens if max_reqs is None else max_reqs
+    if max_tokens < 1 or max_reqs < 0 or n_kv < 1 or not 1 <= G <= 16 or head_dim not in (64, 128, 256):
+        raise ValueError(f"max_tokens {max_tokens}, max_reqs {max_reqs}, n_kv {n_kv}, G {G}, head_dim {head_dim}: need "
+                         "positive counts, G in [1, 16], head_dim 64, 128 or 256")
+    n = _lib.load().locks_attn_workspace_bytes(int(max_reqs), int(max_tokens), int(n_kv), int(G), int(head_dim))
     return torch.empty(n, dtype=torch.uint8, device=device)
 
 

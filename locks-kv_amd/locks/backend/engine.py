@@ -20,7 +20,12 @@ integration spreads this over:
   prologue runs its per-step lifecycle (tier.py:239-301), ``write_kv``
   copies each layer's new V (K) into the staging pool (tier.py:386-392),
   and ``forward`` runs the layer's residency step between selection and the
-  decode, which then reads V (K) through ``TierVSource``.
+  decode, which then reads V (K) through ``TierVSource``;
+* around the selected layers, for an engine without kernels of its own:
+  ``block_tables`` (the step's tables and slots from the requests' lengths),
+  ``write_qkv`` (norm, rotation and cache write of a layer's projection),
+  ``forward_dense`` (prompt chunks and mixed batches, and layers that keep a
+  window) and ``forward_prefix`` (decode of requests on a shared prefix).
 
 A vLLM-ROCm attention backend calls ``prologue`` from its metadata builder
 and ``forward`` from its impl; any other engine can drive it directly.
@@ -29,11 +34,13 @@ from __future__ import annotations
 
 import torch
 
+from ..attention import attn_workspace, prefix_decode, qk_norm_rope_write, window_decode, window_prefill
 from ..attention.decode import _split_kv, ensure_stage_b_buffers
 from ..selection import Rki4State, derive_page_params
 from ..tier import Tier
 from . import _runtime
 from .refresh import RefreshGate
+from .tables import BlockTables
 
 
 class LocksEngine:
@@ -63,12 +70,16 @@ class LocksEngine:
         self.st._layer_of = {kv.data_ptr(): i for i, kv in enumerate(self.kv_caches)}
         self.k_layers = [_split_kv(kv)[0] for kv in self.kv_caches]
         self.gate = RefreshGate(page)
+        self.max_tokens = int(max_num_batched_tokens)
+        self._dense_ws = None
+        self._k_out = None
         self.tier = None
         if cfg.is_mem:
             self.tier = Tier.from_config(
                 cfg, num_layers=len(self.kv_caches), num_blocks=int(K0.shape[0]),
                 n_kv=int(num_heads_kv), page=page, d=int(head_dim), max_reqs=int(max_num_seqs),
                 max_pages=self.st.max_pages, max_tokens=int(max_num_batched_tokens), device=dev)
+            self._k_out = torch.empty(self.max_tokens, int(num_heads_kv), int(head_dim), dtype=torch.bfloat16, device=dev)
 
     @torch.no_grad()
     def prologue(self, block_table, seq_lens, query_start_loc, n_req: int,
@@ -113,3 +124,61 @@ class LocksEngine:
         A no-op for the resident variant."""
         if self.tier is not None:
             self.tier.write_kv(layer, value, key)
+
+    # ---- around the selected layers ------------------------------------------
+    def block_tables(self, reserved: int = 0) -> BlockTables:
+        """Block tables for this engine's cache and limits: ``step`` gives
+        ``prologue`` and the layers their block table, lengths and slots."""
+        return BlockTables(self.kv_caches[0].device, num_blocks=self.st.NB, page=self.st.page,
+                           max_reqs=self.st.max_reqs, max_pages=self.st.max_pages, max_tokens=self.max_tokens,
+                           reserved=reserved)
+
+    @torch.no_grad()
+    def write_qkv(self, layer: int, q, k, v, positions, slot_mapping, cos_sin, q_out, *, n_tokens: int = None,
+                  q_weight=None, k_weight=None, eps: float = 1e-6, interleaved: bool = False) -> None:
+        """A layer's projection made ready (``qk_norm_rope_write``): queries to
+        ``q_out``, keys and values to the layer's cache and, for the mem variants,
+        to the tier's staging pool (``write_kv``)."""
+        n = int(q.shape[0] if n_tokens is None else n_tokens)
+        qk_norm_rope_write(q, k, v, positions, slot_mapping, self.kv_caches[layer], cos_sin, q_out, n_tokens=n,
+                           q_weight=q_weight, k_weight=k_weight, eps=eps, interleaved=interleaved, k_out=self._k_out)
+        if self.tier is not None:
+            self.write_kv(layer, self._k_out[:n], v[:n])
+
+    def _ws(self):
+        """Workspace of the dense calls, made by the first of them (a captured
+        step is run once before its capture)."""
+        if self._dense_ws is None:
+            st = self.st
+            self._dense_ws = attn_workspace(self.kv_caches[0].device, max_tokens=self.max_tokens,
+                                            max_reqs=st.max_reqs, n_kv=st.n_kv, G=st.G, head_dim=st.D)
+        return self._dense_ws
+
+    @torch.no_grad()
+    def forward_dense(self, q, kv_cache, block_table, seq_lens, n_req: int, scale: float, out, *,
+                      query_start_loc=None, n_decode: int = None, n_tokens: int = None, window: int = 0, sinks: int = 0,
+                      lse=None) -> None:
+        """One layer of any step with attention over the whole row, or over the
+        last ``window`` tokens and the first ``sinks``, read from the paged cache.
+        The first ``n_decode`` requests have one new token each (default: all,
+        without ``query_start_loc``; none with it), the others the rows that
+        ``query_start_loc`` gives."""
+        if n_decode is None:
+            n_decode = n_req if query_start_loc is None else 0
+        if not 0 <= n_decode <= n_req or (n_decode < n_req and query_start_loc is None):
+            raise ValueError(f"n_decode {n_decode} of {n_req} requests"
+                             + ("" if query_start_loc is not None else " and no query_start_loc"))
+        kw = dict(scale=scale, window=window, sinks=sinks, lse=lse)
+        if n_decode:
+            window_decode(q, kv_cache, block_table, seq_lens, out, self._ws(), n_req=n_decode, **kw)
+        if n_decode < n_req:
+            window_prefill(q, kv_cache, block_table[n_decode:], seq_lens[n_decode:], query_start_loc[n_decode:], out,
+                           self._ws(), n_req=n_req - n_decode, n_tokens=n_tokens, **kw)
+
+    @torch.no_grad()
+    def forward_prefix(self, q, kv_cache, block_table, seq_lens, group_start, prefix_pages, n_req: int, n_groups: int,
+                       scale: float, out, *, max_prefix_pages: int = 0, lse=None) -> None:
+        """One layer of a single-token step over the whole rows of requests that
+        share their first pages (``prefix_decode``)."""
+        prefix_decode(q, kv_cache, block_table, seq_lens, group_start, prefix_pages, out, self._ws(), n_req=n_req,
+                      n_groups=n_groups, scale=scale, max_prefix_pages=max_prefix_pages, lse=lse)

@@ -391,7 +391,7 @@ def test_refusals():
         for bad in valued:                                   # the last: on the CPU
             with pytest.raises(ValueError):
                 fn(**{**ok, **extra, **bad})
-    for bad in (dict(max_tokens=0), dict(n_kv=0), dict(G=17), dict(head_dim=96)):
+    for bad in (dict(max_tokens=0), dict(max_reqs=-1), dict(n_kv=0), dict(G=17), dict(head_dim=96)):
         with pytest.raises(ValueError):
             attn_workspace("cpu", **{**dict(max_tokens=2, n_kv=2, G=4, head_dim=128), **bad})
 
@@ -431,5 +431,5 @@ def test_workspace_covers_every_call():
     """The bytes grow with the tokens, so a workspace of more covers fewer."""
     lib = _lib.load()
     for n_kv, G, d in ((8, 4, 128), (1, 16, 64), (2, 3, 256)):
-        b = [lib.locks_attn_workspace_bytes(n, n_kv, G, d) for n in (1, 2, 7, 64, 65, 300, 5000)]
+        b = [lib.locks_attn_workspace_bytes(n, n, n_kv, G, d) for n in (1, 2, 7, 64, 65, 300, 5000)]
         assert b == sorted(b) and b[0] > 0
