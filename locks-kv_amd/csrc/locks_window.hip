@@ -70,7 +70,7 @@ struct TileArgs {
 };
 
 // 16 bytes per lane from its own address to 1 KB of LDS, in lane order
-__device__ __forceinline__ void load_lds16(const uint16_t* src, uint8_t* dst) {
+__device__ __forceinline__ void load_lds16(const uint8_t* src, uint8_t* dst) {
     __builtin_amdgcn_global_load_lds(src, (lds_ptr)dst, 16, 0, 0);
 }
 __device__ __forceinline__ int wave_max_int(int v) { return (int)(wave_max_u32((uint32_t)v ^ 0x80000000u) ^ 0x80000000u); }
@@ -87,6 +87,7 @@ __global__ __launch_bounds__(AT_BLK, D == 256 ? 1 : 2) void attn_tile_kernel(con
 {
     using GM = AtGeom<D>;
     constexpr int KT = GM::KT, ROWB = GM::ROWB, NB2 = KT / 32, ND = D / 32;
+    constexpr int VPRE = D == 256 ? ND / 2 : ND;        // column blocks of V read before the softmax
     static_assert(!SHARED || PART, "a prefix is one part of a row");
     __shared__ __attribute__((aligned(1024))) uint8_t k0[GM::TILEB], k1[GM::TILEB], v0[GM::TILEB], v1[GM::TILEB];
     __shared__ int wlim[AT_WAVES][4];
@@ -145,8 +146,10 @@ __global__ __launch_bounds__(AT_BLK, D == 256 ? 1 : 2) void attn_tile_kernel(con
     }
     if (!valid) { hi = 0x7fffffff; lo = 0; }
     // of the wave's valid rows, then of the workgroup's
-    const int w_min_hi = wave_min_int(hi), w_max_hi = wave_max_int(valid ? hi : 0);
-    const int w_max_lo = wave_max_int(lo), w_min_lo = wave_min_int(valid ? lo : 0x7fffffff);
+    const int w_min_hi = __builtin_amdgcn_readfirstlane(wave_min_int(hi));
+    const int w_max_hi = __builtin_amdgcn_readfirstlane(wave_max_int(valid ? hi : 0));
+    const int w_max_lo = __builtin_amdgcn_readfirstlane(wave_max_int(lo));
+    const int w_min_lo = __builtin_amdgcn_readfirstlane(wave_min_int(valid ? lo : 0x7fffffff));
     if (lane == 0) {
         wlim[wave][0] = w_min_hi; wlim[wave][1] = w_max_hi; wlim[wave][2] = w_max_lo; wlim[wave][3] = w_min_lo;
     }
@@ -189,20 +192,25 @@ __global__ __launch_bounds__(AT_BLK, D == 256 ? 1 : 2) void attn_tile_kernel(con
         const int pg = min(min(key >> a.pg_sh, last_page), a.bt_cols - 1);
         ids = min(max(a.bt[bt_row * a.bt_sr + pg], 0), a.NB - 1);
     };
+    // byte offsets of this lane's 16-byte chunks from the wave's first row
+    uint32_t ko[GM::NI], vo[GM::NI];
+#pragma unroll
+    for (int i = 0; i < GM::NI; ++i) {
+        const int at = i * 1024 + lane * 16, row = at / ROWB, slot = (at % ROWB) / 16;
+        const int tr = wave * GM::WROWS + row;              // row of the tile
+        ko[i] = (uint32_t)(row * a.k_st * 2) + 16 * (slot ^ GM::swz_k(tr));
+        vo[i] = (uint32_t)(row * a.v_st * 2) + 16 * (slot ^ GM::swz_v(tr));
+    }
     auto stage = [&](int n, uint8_t* kb, uint8_t* vb) {
         if (n - ids0 >= kWave) fetch_ids(n);
         const long blk = __builtin_amdgcn_readlane(ids, n - ids0);
         const int off = (key_of(n) + wave * GM::WROWS) & ((1 << a.pg_sh) - 1);
-        const uint16_t* kp = a.k + blk * a.k_sb + (long)kh * a.k_sh;
-        const uint16_t* vp = a.v + blk * a.v_sb + (long)kh * a.v_sh;
+        const uint8_t* kp = reinterpret_cast<const uint8_t*>(a.k + blk * a.k_sb + (long)kh * a.k_sh + off * a.k_st);
+        const uint8_t* vp = reinterpret_cast<const uint8_t*>(a.v + blk * a.v_sb + (long)kh * a.v_sh + off * a.v_st);
 #pragma unroll
         for (int i = 0; i < GM::NI; ++i) {
-            const int o = i * 1024 + lane * 16, row = o / ROWB, slot = (o % ROWB) / 16;
-            const int tr = wave * GM::WROWS + row;          // row of the tile
-            load_lds16(kp + (long)(off + row) * a.k_st + 8 * (slot ^ GM::swz_k(tr)),
-                       kb + wave * GM::WROWS * ROWB + i * 1024);
-            load_lds16(vp + (long)(off + row) * a.v_st + 8 * (slot ^ GM::swz_v(tr)),
-                       vb + wave * GM::WROWS * ROWB + i * 1024);
+            load_lds16(kp + ko[i], kb + wave * GM::WROWS * ROWB + i * 1024);
+            load_lds16(vp + vo[i], vb + wave * GM::WROWS * ROWB + i * 1024);
         }
     };
 
@@ -225,20 +233,110 @@ __global__ __launch_bounds__(AT_BLK, D == 256 ? 1 : 2) void attn_tile_kernel(con
         va[b] = row * ROWB + (chunk ^ GM::swz_v(row)) * 16 + (i16 & 1) * 8;
     }
 
-    // S^T of a tile, the running maximum and sum, O^T rescaled; P in bf16 (half a
-    // step 2^-8 of each weight; l keeps the unrounded ones) as PV's operand
-    auto score = [&](int key0, const uint8_t* kb, v8bf* pf) {
-        v16f s[NB2];
+    // S^T of a tile: every K read first, then the products (left to itself the
+    // compiler waits for each read before its product)
+    auto scores = [&](const uint8_t* kb, v16f* s) {
+        v8bf kf[NB2][D / 16];
+#pragma unroll
+        for (int kb2 = 0; kb2 < NB2; ++kb2)
+#pragma unroll
+            for (int st = 0; st < D / 16; ++st)
+                kf[kb2][st] = *reinterpret_cast<const v8bf*>(kb + ka[st] + kb2 * 32 * ROWB);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int kb2 = 0; kb2 < NB2; ++kb2) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[kb2][i] = 0.f;
 #pragma unroll
-            for (int st = 0; st < D / 16; ++st) {
-                const v8bf x = *reinterpret_cast<const v8bf*>(kb + ka[st] + kb2 * 32 * ROWB);
-                s[kb2] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, qf[st], s[kb2], 0, 0, 0);
+            for (int st = 0; st < D / 16; ++st)
+                s[kb2] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[kb2][st], qf[st], s[kb2], 0, 0, 0);
+        }
+    };
+    // The running maximum and sum, O^T rescaled where a maximum grew; P in bf16
+    // (half a step 2^-8 of each weight; l keeps the unrounded ones), PV's operand
+    auto weights = [&](const v16f* s, v8bf* pf) {
+        float mx = s[0][0];
+#pragma unroll
+        for (int kb2 = 0; kb2 < NB2; ++kb2)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[kb2][i]);
+        mx = xor32_max(mx);
+        if (__any(mx > m)) {
+            const float m_new = fmaxf(m, mx);
+            // not below the smallest normal number: 0 x inf would turn an infinite
+            // value's sum into NaN
+            const float alpha = fmaxf(__builtin_amdgcn_exp2f((m - m_new) * a.c), 1.17549435e-38f);
+            m = m_new;
+            l *= alpha;
+#pragma unroll
+            for (int b = 0; b < ND; ++b) o[b] *= alpha;
+        }
+        const float mc = m == -INFINITY ? 0.f : m * a.c;
+#pragma unroll
+        for (int kb2 = 0; kb2 < NB2; ++kb2)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float p = __builtin_amdgcn_exp2f(fmaf(s[kb2][i], a.c, -mc));
+                l += p;
+                pf[2 * kb2 + (i >> 3)][i & 7] = (__bf16)p;
+            }
+    };
+    auto v_frag = [&](const uint8_t* vb, int b, int c) {
+        const uint8_t* x = vb + va[b] + 16 * c * ROWB;
+        const v4s x0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)(x));
+        const v4s x1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)(x + 8 * ROWB));
+        return __builtin_bit_cast(v8bf, __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7));
+    };
+    // A tile that some row sees only part of: masked places of V must not reach the
+    // sums (0 x NaN), whatever an unwritten page or a later token holds.  Values
+    // that are not finite are added to the rows that see them (any weight leaves
+    // them what they are) and count as zero in the product.
+    auto make_finite = [&](int key0, bool live, uint8_t* vb) {
+        uint4* mine = reinterpret_cast<uint4*>(vb) + tid;
+        uint32_t any = 0;
+#pragma unroll
+        for (int i = 0; i < GM::TILEB / 16 / AT_BLK; ++i) {
+            const uint4 x = mine[i * AT_BLK];
+            any |= nonfinite2(x.x) | nonfinite2(x.y) | nonfinite2(x.z) | nonfinite2(x.w);
+        }
+        if (!__syncthreads_or(any != 0)) return;
+        if (live) {
+            for (int kk = 0; kk < KT; ++kk) {
+                const int key = key0 + kk;
+                const bool seen = valid && key < hi && (key >= lo || key < sinks);
+#pragma unroll
+                for (int b = 0; b < ND; ++b)
+#pragma unroll
+                    for (int q4 = 0; q4 < 4; ++q4) {
+                        const uint2 x = *reinterpret_cast<const uint2*>(
+                            vb + kk * ROWB + ((4 * b + q4) ^ GM::swz_v(kk)) * 16 + 8 * h);
+                        if (seen && (nonfinite2(x.x) | nonfinite2(x.y))) {
+                            const float y[4] = {bf16lo(x.x), bf16hi(x.x), bf16lo(x.y), bf16hi(x.y)};
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) o[b][4 * q4 + e] += fabsf(y[e]) <= 3.4e38f ? 0.f : y[e];
+                        }
+                    }
             }
         }
+        __syncthreads();
+        for (int i = 0; i < GM::TILEB / 16 / AT_BLK; ++i) {
+            uint32_t* x = reinterpret_cast<uint32_t*>(mine + i * AT_BLK);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t y = x[e];
+                x[e] = y & ((nonfinite2(y) & 1 ? 0u : 0xFFFFu) | (nonfinite2(y) & 2 ? 0u : 0xFFFF0000u));
+            }
+        }
+        __syncthreads();
+    };
+    auto compute = [&](int n, const uint8_t* kb, uint8_t* vb) {
+        const int key0 = key_of(n);
+        const bool live = key0 < w_max_hi && (key0 + KT > w_min_lo || key0 < sinks);
+        if (key0 + KT > min_hi || (key0 < max_lo && key0 + KT > sinks)) make_finite(key0, live, vb);
+        if (!live) return;                              // nothing for this wave's rows
+        v16f s[NB2];
+        scores(kb, s);
+        __builtin_amdgcn_sched_barrier(0);
         if (key0 + KT > w_min_hi || (key0 < w_max_lo && key0 + KT > sinks)) {
 #pragma unroll
             for (int kb2 = 0; kb2 < NB2; ++kb2)
@@ -249,91 +347,22 @@ __global__ __launch_bounds__(AT_BLK, D == 256 ? 1 : 2) void attn_tile_kernel(con
                     s[kb2][i] = seen ? s[kb2][i] : -INFINITY;
                 }
         }
-        float mx = s[0][0];
+        v8bf vf[ND][KT / 16], pf[KT / 16];
 #pragma unroll
-        for (int kb2 = 0; kb2 < NB2; ++kb2)
+        for (int b = 0; b < VPRE; ++b)                  // on the way during the softmax
 #pragma unroll
-            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[kb2][i]);
-        mx = xor32_max(mx);
-        const float m_new = fmaxf(m, mx);
-        const float mc = m_new == -INFINITY ? 0.f : m_new * a.c;
-        const float alpha = __builtin_amdgcn_exp2f(m * a.c - mc);
-        m = m_new;
-        l *= alpha;
+            for (int c = 0; c < KT / 16; ++c) vf[b][c] = v_frag(vb, b, c);
+        __builtin_amdgcn_sched_barrier(0);
+        weights(s, pf);
 #pragma unroll
-        for (int b = 0; b < ND; ++b) o[b] *= alpha;
+        for (int b = VPRE; b < ND; ++b)
 #pragma unroll
-        for (int kb2 = 0; kb2 < NB2; ++kb2)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const float p = __builtin_amdgcn_exp2f(fmaf(s[kb2][i], a.c, -mc));
-                l += p;
-                pf[2 * kb2 + (i >> 3)][i & 7] = (__bf16)p;
-            }
-    };
-    auto compute = [&](int n, const uint8_t* kb, uint8_t* vb) {
-        const int key0 = key_of(n);
-        // A tile that some row sees only part of: masked places of V must not
-        // reach the sums (0 x NaN), whatever an unwritten page or a later token
-        // holds.  Values that are not finite are added to the rows that see them
-        // (any weight leaves them what they are) and count as zero in the product.
-        bool bad = false;
-        uint4* mine = reinterpret_cast<uint4*>(vb) + tid;
-        if (key0 + KT > min_hi || (key0 < max_lo && key0 + KT > sinks)) {
-            uint32_t any = 0;
-#pragma unroll
-            for (int i = 0; i < GM::TILEB / 16 / AT_BLK; ++i) {
-                const uint4 x = mine[i * AT_BLK];
-                any |= nonfinite2(x.x) | nonfinite2(x.y) | nonfinite2(x.z) | nonfinite2(x.w);
-            }
-            bad = __syncthreads_or(any != 0);
-        }
-        // nothing for this wave's rows in the tile
-        const bool live = key0 < w_max_hi && (key0 + KT > w_min_lo || key0 < sinks);
-        if (!bad && !live) return;
-        v8bf pf[KT / 16];
-        if (live) score(key0, kb, pf);
-        if (bad) {
-            if (live) {
-                for (int kk = 0; kk < KT; ++kk) {
-                    const int key = key0 + kk;
-                    const bool seen = valid && key < hi && (key >= lo || key < sinks);
-#pragma unroll
-                    for (int b = 0; b < ND; ++b)
-#pragma unroll
-                        for (int q4 = 0; q4 < 4; ++q4) {
-                            const uint2 x = *reinterpret_cast<const uint2*>(
-                                vb + kk * ROWB + ((4 * b + q4) ^ GM::swz_v(kk)) * 16 + 8 * h);
-                            if (seen && (nonfinite2(x.x) | nonfinite2(x.y))) {
-                                const float y[4] = {bf16lo(x.x), bf16hi(x.x), bf16lo(x.y), bf16hi(x.y)};
-#pragma unroll
-                                for (int e = 0; e < 4; ++e) o[b][4 * q4 + e] += fabsf(y[e]) <= 3.4e38f ? 0.f : y[e];
-                            }
-                        }
-                }
-            }
-            __syncthreads();
-            for (int i = 0; i < GM::TILEB / 16 / AT_BLK; ++i) {
-                uint32_t* x = reinterpret_cast<uint32_t*>(mine + i * AT_BLK);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const uint32_t y = x[e];
-                    x[e] = y & ((nonfinite2(y) & 1 ? 0u : 0xFFFFu) | (nonfinite2(y) & 2 ? 0u : 0xFFFF0000u));
-                }
-            }
-            __syncthreads();
-            if (!live) return;
-        }
+            for (int c = 0; c < KT / 16; ++c) vf[b][c] = v_frag(vb, b, c);
 #pragma unroll
         for (int b = 0; b < ND; ++b)
 #pragma unroll
-            for (int c = 0; c < KT / 16; ++c) {
-                const uint8_t* x = vb + va[b] + 16 * c * ROWB;
-                const v4s x0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)(x));
-                const v4s x1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)(x + 8 * ROWB));
-                const auto vt = __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7);
-                o[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, vt), pf[c], o[b], 0, 0, 0);
-            }
+            for (int c = 0; c < KT / 16; ++c)
+                o[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[b][c], pf[c], o[b], 0, 0, 0);
     };
     auto arrived = [&]() {
         __builtin_amdgcn_s_waitcnt(0x0F70);             // vmcnt(0): this wave's part of the tile is in LDS
@@ -512,6 +541,8 @@ static int32_t check_attn(const char* what, const uint16_t* q, int64_t q_st, int
     LOCKS_REQUIRE(q && k && v && bt && seq_lens && out, "%s: null pointer argument", what);
     for (int64_t x : {q_st, q_sh, ks[0], ks[1], ks[2], vs[0], vs[1], vs[2]})
         LOCKS_REQUIRE(x % 8 == 0, "%s: q/K/V strides must be multiples of 8 elements (16-byte loads)", what);
+    for (int64_t x : {ks[1], vs[1]})
+        LOCKS_REQUIRE(x >= 0 && x < (1 << 24), "%s: K/V token strides must be in [0, 2^24) elements", what);
     LOCKS_REQUIRE(o_st % 4 == 0 && o_sh % 4 == 0, "%s: out strides must be multiples of 4 elements", what);
     LOCKS_REQUIRE((uintptr_t)q % 16 == 0 && (uintptr_t)k % 16 == 0 && (uintptr_t)v % 16 == 0 && (uintptr_t)out % 8 == 0,
                   "%s: q, K and V must be 16-byte aligned, out 8-byte", what);

@@ -6,7 +6,6 @@ library.  If the library is missing the import of any hot-path entry raises
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import os
 
@@ -165,14 +164,17 @@ def rows_arg(st) -> int:
     return 0 if rb is None else _c.addressof(rb)
 
 
-_SAME = contextlib.nullcontext()
-
-
-def on_device(device):
-    """A context in which `device` (a torch.device with an index) is the current
-    one: a launch goes to the device of its tensors, whichever is current."""
+def launch(fn, what: str, index: int, args: tuple) -> None:
+    """fn(*args, stream) on device `index` and its current stream, whichever
+    device is the current one; raises where it refuses."""
     import torch
-    return _SAME if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    if index == torch._C._cuda_getDevice():
+        rc = fn(*args, stream_ptr(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, stream_ptr(index))
+    if rc:
+        check(rc, what)
 
 
 def stream_ptr(device=None) -> int:
@@ -185,6 +187,8 @@ def stream_ptr(device=None) -> int:
         return int(torch.cuda.current_stream(device).cuda_stream)
     if device is None:
         return raw(torch.cuda.current_device())
+    if type(device) is int:
+        return raw(device)
     d = torch.device(device)
     if d.type != "cuda":
         raise ValueError(f"Expected a cuda device, but got: {d}")

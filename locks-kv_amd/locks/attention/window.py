@@ -26,25 +26,27 @@ def attn_workspace(device, *, max_tokens: int, n_kv: int, G: int, head_dim: int,
     return torch.empty(n, dtype=torch.uint8, device=device)
 
 
-def _i32(name: str, t, n: int, device) -> None:
-    if t.dtype != torch.int32 or t.dim() != 1 or (t.numel() > 1 and t.stride(0) != 1):
+_BF16, _I32, _F32 = torch.bfloat16, torch.int32, torch.float32
+
+
+def _i32(name: str, t, n: int, index: int) -> None:
+    if t.dtype is not _I32 or t.dim() != 1 or (t.numel() > 1 and t.stride(0) != 1):
         raise TypeError(f"{name} must be a contiguous int32 vector, got {t.dtype} {tuple(t.shape)}")
-    if t.shape[0] < n or t.device != device:
-        raise ValueError(f"{name} must hold {n} entries on {device}, got {t.shape[0]} on {t.device}")
+    if t.shape[0] < n or t.get_device() != index:
+        raise ValueError(f"{name} must hold {n} entries on the cache's device, got {t.shape[0]} on {t.device}")
 
 
-def _args(what: str, q, kv_cache, block_table, seq_lens, out, ws, lse, rows: int, n_req: int):
-    """The checks that the calls share, and their common arguments: (head, of q
-    up to seq_lens; tail, from out to the workspace; n_kv, G, d, page; device)."""
-    if kv_cache.dim() != 5 or kv_cache.dtype != torch.bfloat16 or kv_cache.stride(-1) != 1:
+def _refuse(what: str, q, kv_cache, block_table, seq_lens, out, ws, lse, rows: int, n_req: int) -> None:
+    """The error of a call that _args does not take."""
+    if kv_cache.dim() != 5 or kv_cache.dtype is not _BF16 or kv_cache.stride(-1) != 1:
         raise TypeError(f"{what}: kv_cache must be a 5-d bf16 cache with a contiguous last dim, got "
                         f"{kv_cache.dtype} {tuple(kv_cache.shape)}")
-    kp, vp, ks, (NB, page, n_kv, d) = _kv_args(kv_cache)
+    _, vp, _, (_, _, n_kv, d) = _kv_args(kv_cache)
     if vp is None:
         raise ValueError(f"{what} needs a cache with a V half")
     dev = kv_cache.device
     for name, t in (("q", q), ("out", out)):
-        if t.dtype != torch.bfloat16 or t.dim() != 3 or t.stride(-1) != 1:
+        if t.dtype is not _BF16 or t.dim() != 3 or t.stride(-1) != 1:
             raise TypeError(f"{what}: {name} must be bf16 (rows, heads, d) with a contiguous last dim, got {t.dtype} "
                             f"{tuple(t.shape)} strides {t.stride()}")
         if t.shape[0] < rows or t.shape[2] != d or t.shape[1] % n_kv or t.shape[1] != q.shape[1]:
@@ -52,29 +54,51 @@ def _args(what: str, q, kv_cache, block_table, seq_lens, out, ws, lse, rows: int
                              f"multiple of {n_kv} heads")
         if t.device != dev:
             raise ValueError(f"{what}: {name} is on {t.device}, the cache on {dev}")
-    H = int(q.shape[1])
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.stride(1) != 1:
+    if block_table.dtype is not _I32 or block_table.dim() != 2 or block_table.stride(1) != 1:
         raise TypeError(f"{what}: block_table must be int32 (requests, pages) with contiguous rows")
     if block_table.shape[0] < n_req or block_table.device != dev:
         raise ValueError(f"{what}: block_table must hold {n_req} rows on {dev}, got {block_table.shape[0]} on "
                          f"{block_table.device}")
-    _i32(f"{what}: seq_lens", seq_lens, n_req, dev)
-    ls = 0
+    _i32(f"{what}: seq_lens", seq_lens, n_req, kv_cache.get_device())
     if lse is not None:
-        if lse.dtype != torch.float32 or lse.dim() != 2 or lse.stride(1) != 1:
+        if lse.dtype is not _F32 or lse.dim() != 2 or lse.stride(1) != 1:
             raise TypeError(f"{what}: lse must be fp32 (rows, heads) with contiguous rows")
-        if lse.shape[0] < rows or lse.shape[1] != H or lse.device != dev:
-            raise ValueError(f"{what}: lse must be ({rows}, {H}) on {dev}, got {tuple(lse.shape)} on {lse.device}")
-        ls = lse.stride(0)
+        raise ValueError(f"{what}: lse must be ({rows}, {q.shape[1]}) on {dev}, got {tuple(lse.shape)} on {lse.device}")
     if ws is not None and (ws.device != dev or not ws.is_contiguous()):
         raise ValueError(f"{what}: the workspace must be contiguous, on {dev}")
-    if dev.type != "cuda":
-        raise ValueError(f"{what} runs on the GPU, the cache is on {dev}")
-    head = (q.data_ptr(), *q.stride()[:2], kp, *ks, vp, *ks, NB, block_table.data_ptr(), block_table.stride(0),
-            int(block_table.shape[1]), seq_lens.data_ptr())
-    tail = (out.data_ptr(), *out.stride()[:2], _lib.ptr(lse), ls, _lib.ptr(ws),
-            0 if ws is None else ws.numel() * ws.element_size())
-    return head, tail, (n_kv, H // n_kv, d, page), dev
+    raise ValueError(f"{what} runs on the GPU, the cache is on {dev}, and n_req {n_req} and the rows {rows} must not "
+                     "be negative")
+
+
+def _args(what: str, q, kv_cache, block_table, seq_lens, out, ws, lse, rows: int, n_req: int):
+    """The checks that the calls share (one pass over the tensors' attributes:
+    with a message at each check they took 7 us of a small call), and their common
+    arguments: of q up to seq_lens; from out to the workspace; n_kv, G, d, page; the
+    device's index."""
+    index = kv_cache.get_device()
+    qs, os, qt, ot, bs, bt = q.shape, out.shape, q.stride(), out.stride(), block_table.shape, block_table.stride()
+    ok = (index >= 0 and kv_cache.dim() == 5 and kv_cache.dtype is _BF16 and q.dtype is _BF16 and out.dtype is _BF16
+          and block_table.dtype is _I32 and seq_lens.dtype is _I32 and len(qs) == 3 and len(os) == 3 and len(bs) == 2
+          and qt[2] == 1 and ot[2] == 1 and bt[1] == 1 and seq_lens.dim() == 1 and seq_lens.is_contiguous()
+          and rows >= 0 and n_req >= 0 and qs[0] >= rows and os[0] >= rows and bs[0] >= n_req
+          and seq_lens.shape[0] >= n_req and q.get_device() == index and out.get_device() == index
+          and block_table.get_device() == index and seq_lens.get_device() == index
+          and (ws is None or (ws.get_device() == index and ws.is_contiguous())))
+    if ok:
+        kp, vp, ks, (NB, page, n_kv, d) = _kv_args(kv_cache)
+        H = qs[1]
+        ok = vp is not None and kv_cache.stride(4) == 1 and H % n_kv == 0 and os[1] == H and qs[2] == d and os[2] == d
+        lp = ls = 0
+        if ok and lse is not None:
+            zs, zt = lse.shape, lse.stride()
+            ok = (lse.dtype is _F32 and len(zs) == 2 and zt[1] == 1 and zs[0] >= rows and zs[1] == H
+                  and lse.get_device() == index)
+            lp, ls = lse.data_ptr(), zt[0]
+    if not ok:
+        _refuse(what, q, kv_cache, block_table, seq_lens, out, ws, lse, rows, n_req)
+    head = (q.data_ptr(), qt[0], qt[1], kp, *ks, vp, *ks, NB, block_table.data_ptr(), bt[0], bs[1], seq_lens.data_ptr())
+    tail = (out.data_ptr(), ot[0], ot[1], lp, ls, *((0, 0) if ws is None else (ws.data_ptr(), ws.nbytes)))
+    return head, tail, (n_kv, H // n_kv, d, page), index
 
 
 def window_decode(q, kv_cache, block_table, seq_lens, out, ws, *, n_req: int, scale: float, window: int = 0,
@@ -85,13 +109,11 @@ def window_decode(q, kv_cache, block_table, seq_lens, out, ws, *, n_req: int, sc
     all), and ``lse[:n_req]`` (T, H) fp32 the log-sum-exp of the scores.  A request
     of length 0 (padding) gives zeros and -inf.  ``max_seq_len``: an upper bound of
     the lengths, where one is known, sizes the launch.  ``ws``: attn_workspace."""
-    head, tail, geo, dev = _args("window_decode", q, kv_cache, block_table, seq_lens, out, ws, lse, n_req, n_req)
+    head, tail, geo, index = _args("window_decode", q, kv_cache, block_table, seq_lens, out, ws, lse, n_req, n_req)
     if n_req == 0:
         return
-    with _lib.on_device(dev):
-        _lib.check(_lib.load().locks_window_decode(*head, int(window), int(sinks), *tail, int(n_req), *geo,
-                                                   int(max_seq_len), float(scale), _lib.stream_ptr(dev)),
-                   "window_decode")
+    _lib.launch(_lib.load().locks_window_decode, "window_decode", index,
+                (*head, window, sinks, *tail, n_req, *geo, max_seq_len, scale))
 
 
 def window_prefill(q, kv_cache, block_table, seq_lens, query_start_loc, out, ws, *, n_req: int, scale: float,
@@ -101,15 +123,13 @@ def window_prefill(q, kv_cache, block_table, seq_lens, query_start_loc, out, ws,
     the keys up to its own position, in the window or among the first ``sinks`` as
     for ``window_decode``.  Rows from ``query_start_loc[n_req]`` on stay as they
     were.  ``n_tokens`` (default: the rows of q) bounds the rows read."""
-    n_tokens = int(q.shape[0] if n_tokens is None else n_tokens)
-    head, tail, geo, dev = _args("window_prefill", q, kv_cache, block_table, seq_lens, out, ws, lse, n_tokens, n_req)
-    _i32("window_prefill: query_start_loc", query_start_loc, n_req + 1, dev)
+    n_tokens = q.shape[0] if n_tokens is None else n_tokens
+    head, tail, geo, index = _args("window_prefill", q, kv_cache, block_table, seq_lens, out, ws, lse, n_tokens, n_req)
+    _i32("window_prefill: query_start_loc", query_start_loc, n_req + 1, index)
     if n_req == 0 or n_tokens == 0:
         return
-    with _lib.on_device(dev):
-        _lib.check(_lib.load().locks_window_prefill(
-            *head, query_start_loc.data_ptr(), int(window), int(sinks), *tail, n_tokens, int(n_req), *geo,
-            int(max_seq_len), float(scale), _lib.stream_ptr(dev)), "window_prefill")
+    _lib.launch(_lib.load().locks_window_prefill, "window_prefill", index,
+                (*head, query_start_loc.data_ptr(), window, sinks, *tail, n_tokens, n_req, *geo, max_seq_len, scale))
 
 
 def prefix_decode(q, kv_cache, block_table, seq_lens, group_start, prefix_pages, out, ws, *, n_req: int,
@@ -120,12 +140,11 @@ def prefix_decode(q, kv_cache, block_table, seq_lens, group_start, prefix_pages,
     the row of its first request.  Both are int32 on the GPU, so that a captured
     call follows them.  Requests outside all groups, members shorter than the
     prefix and padding (length 0) are attended like any other."""
-    head, tail, geo, dev = _args("prefix_decode", q, kv_cache, block_table, seq_lens, out, ws, lse, n_req, n_req)
-    _i32("prefix_decode: group_start", group_start, n_groups + 1, dev)
-    _i32("prefix_decode: prefix_pages", prefix_pages, n_groups, dev)
+    head, tail, geo, index = _args("prefix_decode", q, kv_cache, block_table, seq_lens, out, ws, lse, n_req, n_req)
+    _i32("prefix_decode: group_start", group_start, n_groups + 1, index)
+    _i32("prefix_decode: prefix_pages", prefix_pages, n_groups, index)
     if n_req == 0:
         return
-    with _lib.on_device(dev):
-        _lib.check(_lib.load().locks_prefix_decode(
-            *head, group_start.data_ptr(), prefix_pages.data_ptr(), int(n_groups), *tail, int(n_req), *geo,
-            int(max_prefix_pages), int(max_seq_len), float(scale), _lib.stream_ptr(dev)), "prefix_decode")
+    _lib.launch(_lib.load().locks_prefix_decode, "prefix_decode", index,
+                (*head, group_start.data_ptr(), prefix_pages.data_ptr(), n_groups, *tail, n_req, *geo, max_prefix_pages,
+                 max_seq_len, scale))

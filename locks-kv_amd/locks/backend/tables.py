@@ -35,7 +35,8 @@ class BlockTables:
 
     Outputs of ``step``: ``block_table`` (max_reqs, max_pages), ``seq_lens``
     (max_reqs,), ``query_start_loc`` (max_reqs + 1,), ``positions`` (max_tokens,)
-    int32 and ``slot_mapping`` (max_tokens,) int64.
+    int32 and ``slot_mapping`` (max_tokens,) int64.  All of these are written in
+    place and never replaced.
     """
 
     def __init__(self, device, *, num_blocks: int, page: int, max_reqs: int, max_pages: int, max_tokens: int,
@@ -65,7 +66,14 @@ class BlockTables:
         self.query_start_loc = torch.zeros(max_reqs + 1, **z)
         self.positions = torch.zeros(max_tokens, **z)
         self.slot_mapping = torch.full((max_tokens,), -1, dtype=torch.int64, device=device)
-        self.device = self.table.device
+        self.device, self._index = self.table.device, self.table.get_device()
+        # what the two entries take of the object's own buffers, which stay where they are
+        pool = (self.lens.data_ptr(), self.table.data_ptr(), self.table.stride(0), self.max_reqs, self.max_pages,
+                self.free.data_ptr(), self.num_blocks, self.state.data_ptr())
+        self._step_args = (*pool, self.block_table.data_ptr(), self.block_table.stride(0), self.seq_lens.data_ptr(),
+                           self.query_start_loc.data_ptr(), self.positions.data_ptr(), self.slot_mapping.data_ptr(),
+                           self.page)
+        self._trim_args = (*pool, self.page)
 
     def set_free(self, head: int) -> None:
         """The free blocks are ``free[head:]`` (for a caller that fills ``free``,
@@ -74,13 +82,16 @@ class BlockTables:
             raise ValueError(f"head {head} outside [0, num_blocks {self.num_blocks}]")
         self.state[0] = int(head)
 
-    def _check(self, name: str, t, n_req: int) -> None:
-        if t.dtype != torch.int32 or t.dim() != 1 or (t.numel() > 1 and t.stride(0) != 1):
+    def _check(self, name: str, t, n_req: int) -> int:
+        """The address of a vector of n_req entries on the tables' device."""
+        if (t.dtype is torch.int32 and t.dim() == 1 and t.is_contiguous() and t.shape[0] >= n_req
+                and t.get_device() == self._index and self._index >= 0):
+            return t.data_ptr()
+        if t.dtype is not torch.int32 or t.dim() != 1 or not t.is_contiguous():
             raise TypeError(f"{name} must be a contiguous int32 vector, got {t.dtype} {tuple(t.shape)}")
-        if t.device != self.device or self.device.type != "cuda":
-            raise ValueError(f"{name} is on {t.device}, the tables on {self.device}")
         if t.shape[0] < n_req:
             raise ValueError(f"{name} has {t.shape[0]} entries for n_req {n_req}")
+        raise ValueError(f"{name} is on {t.device}, the tables on {self.device}: both must be on one GPU")
 
     def step(self, rows, new_lens, n_req: int, n_tokens: int) -> None:
         """The step of requests ``rows[:n_req]`` (distinct rows; -1 pads the
@@ -100,15 +111,8 @@ class BlockTables:
             raise ValueError(f"n_req {n_req} outside [0, max_reqs {self.max_reqs}]")
         if not 0 <= n_tokens <= self.max_tokens:
             raise ValueError(f"n_tokens {n_tokens} outside [0, max_tokens {self.max_tokens}]")
-        self._check("rows", rows, n_req)
-        self._check("new_lens", new_lens, n_req)
-        with _lib.on_device(self.device):
-            _lib.check(_lib.load().locks_tables_step(
-                rows.data_ptr(), new_lens.data_ptr(), n_req, n_tokens, self.lens.data_ptr(), self.table.data_ptr(),
-                self.table.stride(0), self.max_reqs, self.max_pages, self.free.data_ptr(), self.num_blocks,
-                self.state.data_ptr(), self.block_table.data_ptr(), self.block_table.stride(0),
-                self.seq_lens.data_ptr(), self.query_start_loc.data_ptr(), self.positions.data_ptr(),
-                self.slot_mapping.data_ptr(), self.page, _lib.stream_ptr(self.device)), "tables_step")
+        _lib.launch(_lib.load().locks_tables_step, "tables_step", self._index, (
+            self._check("rows", rows, n_req), self._check("new_lens", new_lens, n_req), n_req, n_tokens, *self._step_args))
 
     def trim(self, rows, keep_lens, n_req: int) -> None:
         """Shorten requests ``rows[:n_req]`` to ``keep_lens`` tokens (0: the
@@ -123,10 +127,5 @@ class BlockTables:
         n_req = int(n_req)
         if not 0 <= n_req <= self.max_reqs:
             raise ValueError(f"n_req {n_req} outside [0, max_reqs {self.max_reqs}]")
-        self._check("rows", rows, n_req)
-        self._check("keep_lens", keep_lens, n_req)
-        with _lib.on_device(self.device):
-            _lib.check(_lib.load().locks_tables_trim(
-                rows.data_ptr(), keep_lens.data_ptr(), n_req, self.lens.data_ptr(), self.table.data_ptr(),
-                self.table.stride(0), self.max_reqs, self.max_pages, self.free.data_ptr(), self.num_blocks,
-                self.state.data_ptr(), self.page, _lib.stream_ptr(self.device)), "tables_trim")
+        _lib.launch(_lib.load().locks_tables_trim, "tables_trim", self._index, (
+            self._check("rows", rows, n_req), self._check("keep_lens", keep_lens, n_req), n_req, *self._trim_args))
