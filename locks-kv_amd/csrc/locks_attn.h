@@ -7,23 +7,23 @@
 namespace locks {
 
 // The keys of a single-token decode over a range of the row's tokens:
-// [lo, seq_len) and [0, min(sinks, lo)), with lo = seq_len - window (0 without a
-// window), or the end of the prefix of the request's group.
+// [lo, seq_len) and [0, min(sinks, lo)), lo = max(seq_len - window, 0) (0 without a
+// window).
 struct RangeSrc {
     int window, sinks;                      // window 0: none
-    const int* gstart; const int* gpages;   // groups [gstart[g], gstart[g + 1]) of requests, their prefix pages
-    int n_groups;                           // 0: no groups
-    int first_split;                        // partials of split s go to first_split + s
 };
 
-// The group of request r (the same in every lane), or -1.
-__device__ __forceinline__ int group_of(const int* __restrict__ gstart, int n_groups, int r) {
+// The prefix pages of request r's group (the same in every lane), or -1.  All loads
+// of 64 groups go out together: a workgroup of a short row lives as long as its
+// chain of dependent loads.
+__device__ __forceinline__ int group_pages(const int* __restrict__ gstart, const int* __restrict__ gpages, int n_groups,
+                                           int r) {
     const int lane = threadIdx.x & 63;
     for (int g0 = 0; g0 < n_groups; g0 += kWave) {
-        const int g = g0 + lane;
-        const bool in = g < n_groups && gstart[g] <= r && r < gstart[g + 1];
-        const unsigned long long m = __ballot(in);
-        if (m) return g0 + __ffsll(m) - 1;
+        const int g = min(g0 + lane, n_groups - 1);
+        const int first = gstart[g], end = gstart[g + 1], pages = gpages[g];
+        const unsigned long long m = __ballot(first <= r && r < end);
+        if (m) return max(__builtin_amdgcn_readlane(pages, __ffsll(m) - 1), 0);
     }
     return -1;
 }

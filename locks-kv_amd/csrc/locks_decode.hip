@@ -311,12 +311,7 @@ __global__ __launch_bounds__(DC_BLK) void decode_split_kernel(
     int lo = 0, sinks = 0, n_sink = 0, t_gap = 0;       // RANGE: first key, first keys; steps of those, steps skipped
     if constexpr (RANGE) {
         const int n = (int)min((long)seq_lens[r], (long)bt_cols * PG);
-        if (tier.n_groups) {
-            const int g = group_of(tier.gstart, tier.n_groups, r);
-            lo = g < 0 ? 0 : (int)min((long)max(tier.gpages[g], 0) * PG, (long)max(n, 0));
-        } else {
-            lo = tier.window ? max(n - tier.window, 0) : 0;
-        }
+        lo = tier.window ? max(n - tier.window, 0) : 0;
         sinks = min(tier.sinks, lo);
         n_sink = (sinks + DC_PG - 1) / DC_PG;
         t_gap = max(lo / DC_PG - n_sink, 0);
@@ -329,14 +324,6 @@ __global__ __launch_bounds__(DC_BLK) void decode_split_kernel(
     }
     // gridDim.x = the launched split count (<= split, the buffers' stride)
     const int nsplit = gridDim.x;
-    if constexpr (RANGE) {
-        // a request in no group has no partials of a prefix
-        if (tier.n_groups && sp == 0 && group_of(tier.gstart, tier.n_groups, r) < 0)
-            for (int i = tid; i < tier.first_split * G; i += DC_BLK) {
-                m_part[rk * split * G + i] = -INFINITY;
-                l_part[rk * split * G + i] = 0.f;
-            }
-    }
     const int pps = max(cdiv(cnt, nsplit), pps_min);
     const int j0 = sp * pps;
     if constexpr (FUSED) {
@@ -352,7 +339,7 @@ __global__ __launch_bounds__(DC_BLK) void decode_split_kernel(
     }
     if constexpr (RANGE) {
         if (j0 >= cnt) {
-            const long i = (rk * split + tier.first_split + sp) * G + tid;
+            const long i = (rk * split + sp) * G + tid;
             if (tid < G) { m_part[i] = -INFINITY; l_part[i] = 0.f; }
             return;
         }
@@ -647,8 +634,7 @@ __global__ __launch_bounds__(DC_BLK) void decode_split_kernel(
                     make_float4(o[4 * j][v], o[4 * j + 1][v], o[4 * j + 2][v], o[4 * j + 3][v]);
     }
     __syncthreads();
-    long base = (rk * split + sp) * G;
-    if constexpr (RANGE) base += (long)tier.first_split * G;
+    const long base = (rk * split + sp) * G;
     for (int i = tid; i < G * (D / 4); i += DC_BLK) {
         const int g = i / (D / 4), d = (i % (D / 4)) * 4;
         float M = wm[0][g];

@@ -21,7 +21,8 @@
 // row are permuted by the row on the way in (an exclusive or), which keeps the
 // reads of both operands free of bank conflicts.
 //
-// Decode (one token): the split kernel of locks_decode.hip over a token range.
+// Decode (one token): the split kernel of locks_decode.hip over a token range, or
+// (with a shared prefix) the tiles above, of which a request fills one column block.
 #include "locks_attn.h"
 #include "locks_common.h"
 #include "locks_hip.h"
@@ -67,6 +68,8 @@ struct TileArgs {
     float c;                                // scale * log2(e)
     float scale;
     int NB, bt_cols, n_rows, n_seq, n_kv, G, pg_sh, window, sinks, nsplit;
+    int own;                                // SHARED: splits of a request's own keys, behind the nsplit of its prefix
+    int shared_units, own_units, chunk;     // and how the two kinds of work are dealt out (per kv head)
 };
 
 // 16 bytes per lane from its own address to 1 KB of LDS, in lane order
@@ -80,7 +83,10 @@ __device__ __forceinline__ uint32_t nonfinite2(uint32_t w) {
     return ((w & 0x7F80u) == 0x7F80u ? 1u : 0u) | ((w & 0x7F800000u) == 0x7F800000u ? 2u : 0u);
 }
 
-// SHARED: rows are the members of a group and the keys its prefix; partials only.
+// SHARED: rows are the members of a group and the keys its prefix, or (the other
+// kind of work in the same launch) the heads of one request and its own keys;
+// partials only.  The prefix is bound by the matrix cores, own keys by memory: dealt
+// out in turns of one workgroup per CU, they overlap.
 // PART: partials instead of the output.
 template <int D, bool SHARED, bool PART>
 __global__ __launch_bounds__(AT_BLK, D == 256 ? 1 : 2) void attn_tile_kernel(const TileArgs a)
@@ -95,13 +101,33 @@ __global__ __launch_bounds__(AT_BLK, D == 256 ? 1 : 2) void attn_tile_kernel(con
     const int c32 = lane & 31, h = lane >> 5;
     const int G = a.G, TQ = AT_ROWS / G;                // tokens per tile
     const int kh = blockIdx.x % a.n_kv;
-    const int rest = blockIdx.x / a.n_kv;
-    const int sp = rest % a.nsplit;
-    const int tile = rest / a.nsplit;
-
-    // the request (group) that holds this tile
+    const int unit = blockIdx.x / a.n_kv;
     int seq = -1, t_in = 0, first = 0, count = 0;
-    for (int s0 = 0, done = 0; s0 < a.n_seq; s0 += kWave) {
+    int sp = unit % a.nsplit, slot = sp, nsplit = a.nsplit, tile = unit / a.nsplit;
+    bool own = false;
+    if constexpr (SHARED) {
+        // turns of `chunk` units of each kind while both last, then what is left
+        const int turns = min(a.shared_units, a.own_units) / a.chunk;
+        const int turn = unit / (2 * a.chunk), at = unit % (2 * a.chunk);
+        int i;
+        if (turn < turns) {
+            own = at >= a.chunk;
+            i = turn * a.chunk + (own ? at - a.chunk : at);
+        } else {
+            i = unit - turns * a.chunk;
+            own = i >= a.shared_units;
+            i = own ? unit - a.shared_units : i;
+        }
+        if (own) {
+            seq = first = i / a.own;
+            count = 1;
+            sp = i % a.own; slot = a.nsplit + sp; nsplit = a.own;
+        } else {
+            sp = slot = i % a.nsplit; tile = i / a.nsplit;
+        }
+    }
+    // the request (group) that holds this tile
+    for (int s0 = 0, done = 0; s0 < a.n_seq && seq < 0; s0 += kWave) {
         const int s = s0 + lane;
         int f = 0, n = 0;
         if (s < a.n_seq) {
@@ -119,7 +145,6 @@ __global__ __launch_bounds__(AT_BLK, D == 256 ? 1 : 2) void attn_tile_kernel(con
             const int nt_l = __builtin_amdgcn_readlane(nt, l);
             // the tiles that see most first
             t_in = nt_l - 1 - (tile - done - (__builtin_amdgcn_readlane(inc, l) - nt_l));
-            break;
         }
         done += __builtin_amdgcn_readlane(inc, 63);
     }
@@ -131,11 +156,22 @@ __global__ __launch_bounds__(AT_BLK, D == 256 ? 1 : 2) void attn_tile_kernel(con
     const int j = t_in * TQ + rho / G, g = rho % G;
     const bool valid = rho < TQ * G && j < count;
     const int tok = first + (valid ? j : 0);
-    int hi, lo = 0, sinks = 0;
+    int hi, lo = 0, sinks = 0, base = 0;                // base: where the key tiles start
     long bt_row;
     if constexpr (SHARED) {
-        const long pre = min((long)max(a.gpages[seq], 0), (long)a.bt_cols) << a.pg_sh;
-        hi = (int)min(pre, (long)a.seq_lens[tok]);
+        const int sl = a.seq_lens[tok];
+        const int pages = own ? group_pages(a.starts, a.gpages, a.n_seq, seq) : max(a.gpages[seq], 0);
+        const long pre = min((long)max(pages, 0), (long)a.bt_cols) << a.pg_sh;
+        hi = (int)min(own ? cap : pre, (long)sl);
+        if (own) {
+            base = lo = (int)min(pre, (long)max(sl, 0));
+            if (pages < 0 && sp == 0 && tid < G)        // a request in no group has no partials of a prefix
+                for (int i = 0; i < a.nsplit; ++i) {
+                    const long at = (((long)tok * a.n_kv + kh) * a.p.splits + i) * G + tid;
+                    a.p.m[at] = -INFINITY;
+                    a.p.l[at] = 0.f;
+                }
+        }
         bt_row = first;
     } else {
         const int pos = a.seq_lens[seq] - (min(a.starts[seq + 1], a.n_rows) - a.starts[seq]) + j;
@@ -165,10 +201,11 @@ __global__ __launch_bounds__(AT_BLK, D == 256 ? 1 : 2) void attn_tile_kernel(con
 
     // key tiles: the first na, then [b0, b1); this split's share of them
     const int na = (min(min(sinks, min_lo), max(max_hi, 0)) + KT - 1) / KT;
-    const int b0 = max(min_lo / KT, na), b1 = (int)(((long)max_hi + KT - 1) / KT);
-    const int nt = max_hi > 0 ? na + max(b1 - b0, 0) : 0;
-    const int n0 = (int)((long)nt * sp / a.nsplit), n1 = (int)((long)nt * (sp + 1) / a.nsplit);
-    auto key_of = [&](int n) { return (n < na ? n : b0 + n - na) * KT; };
+    base = __builtin_amdgcn_readfirstlane(base);
+    const int b0 = max((min_lo - base) / KT, na), b1 = (int)(((long)max_hi - base + KT - 1) / KT);
+    const int nt = max_hi > base ? na + max(b1 - b0, 0) : 0;
+    const int n0 = (int)((long)nt * sp / nsplit), n1 = (int)((long)nt * (sp + 1) / nsplit);
+    auto key_of = [&](int n) { return base + (n < na ? n : b0 + n - na) * KT; };
 
     // Q: k-slots 8 h .. 8 h + 7 of MFMA step s are d = 16 s + 8 h ..
     v8bf qf[D / 16];
@@ -244,13 +281,14 @@ __global__ __launch_bounds__(AT_BLK, D == 256 ? 1 : 2) void attn_tile_kernel(con
                 kf[kb2][st] = *reinterpret_cast<const v8bf*>(kb + ka[st] + kb2 * 32 * ROWB);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int kb2 = 0; kb2 < NB2; ++kb2) {
+        for (int kb2 = 0; kb2 < NB2; ++kb2)
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[kb2][i] = 0.f;
 #pragma unroll
-            for (int st = 0; st < D / 16; ++st)
+        for (int st = 0; st < D / 16; ++st)
+#pragma unroll
+            for (int kb2 = 0; kb2 < NB2; ++kb2)
                 s[kb2] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[kb2][st], qf[st], s[kb2], 0, 0, 0);
-        }
     };
     // The running maximum and sum, O^T rescaled where a maximum grew; P in bf16
     // (half a step 2^-8 of each weight; l keeps the unrounded ones), PV's operand
@@ -261,7 +299,9 @@ __global__ __launch_bounds__(AT_BLK, D == 256 ? 1 : 2) void attn_tile_kernel(con
 #pragma unroll
             for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[kb2][i]);
         mx = xor32_max(mx);
-        if (__any(mx > m)) {
+        // m follows the maximum only when it has grown by 2^8 in weight: until then
+        // the weights are at most 256, and o and l need no rescaling
+        if (__any((mx - m) * a.c > 8.f)) {
             const float m_new = fmaxf(m, mx);
             // not below the smallest normal number: 0 x inf would turn an infinite
             // value's sum into NaN
@@ -359,9 +399,9 @@ __global__ __launch_bounds__(AT_BLK, D == 256 ? 1 : 2) void attn_tile_kernel(con
 #pragma unroll
             for (int c = 0; c < KT / 16; ++c) vf[b][c] = v_frag(vb, b, c);
 #pragma unroll
-        for (int b = 0; b < ND; ++b)
+        for (int c = 0; c < KT / 16; ++c)
 #pragma unroll
-            for (int c = 0; c < KT / 16; ++c)
+            for (int b = 0; b < ND; ++b)
                 o[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[b][c], pf[c], o[b], 0, 0, 0);
     };
     auto arrived = [&]() {
@@ -385,7 +425,7 @@ __global__ __launch_bounds__(AT_BLK, D == 256 ? 1 : 2) void attn_tile_kernel(con
     l = xor32_sum(l);
     if (!valid) return;
     if constexpr (PART) {
-        const long at = (((long)tok * a.n_kv + kh) * a.p.splits + sp) * G + g;
+        const long at = (((long)tok * a.n_kv + kh) * a.p.splits + slot) * G + g;
         if (h == 0) {
             a.p.m[at] = l > 0.f || l != l ? m * a.scale : -INFINITY;
             a.p.l[at] = l;
@@ -484,12 +524,20 @@ __global__ __launch_bounds__(AM_BLK) void attn_merge_kernel(const Partials p, ui
 static int clampi(long x, int lo, int hi) { return (int)(x < lo ? lo : x > hi ? hi : x); }
 
 // A single-token call: about 512 workgroups (two per CU), each of at least 8
-// 16-token steps (two per wave).
-static int decode_splits(int n_req, int n_kv, long max_keys) {
+// 16-token steps (two per wave).  With `even`, a row's splits hold at most 64 steps:
+// lengths differ, and the longest split is the call's time (32 ragged requests of a
+// window of 8192: 119 us at 2 splits, 96.5 at 9, 103 at 17).
+static int decode_splits(int n_req, int n_kv, long max_keys, bool even) {
     const long rows = (long)n_req * n_kv, steps = (max_keys + 15) / 16;
-    return clampi((512 + rows - 1) / rows, 1, clampi((steps + 7) / 8, 1, 64));
+    const long fill = (512 + rows - 1) / rows, most = even ? (steps + 63) / 64 : 1;
+    return clampi(fill > most ? fill : most, 1, clampi((steps + 7) / 8, 1, 64));
 }
-static long prefill_tiles(int n_tokens, int n_req, int G) { return (long)n_tokens / (AT_ROWS / G) + n_req; }
+// Tiles of k non-empty requests (groups) of n tokens together: sum of ceil(c / TQ)
+// <= floor((n - k) / TQ) + k, largest where all are non-empty.
+static long prefill_tiles(int n_tokens, int n_req, int G) {
+    const int k = n_req < n_tokens ? n_req : n_tokens;
+    return (long)(n_tokens - k) / (AT_ROWS / G) + k;
+}
 // Many tokens: one split once there are 256 workgroups, else about 512 of at
 // least 4 key tiles.
 static int prefill_splits(long tiles, int n_kv, long max_keys, int head_dim) {
@@ -569,7 +617,9 @@ extern "C" int64_t locks_attn_workspace_bytes(int32_t max_reqs, int32_t max_toke
     // single-token calls of up to max_reqs requests, with a prefix (of one group:
     // more of them make fewer splits); calls of many tokens, of one request (ditto)
     for (int n = 1; n <= (max_reqs < 65535 ? max_reqs : 65535); ++n) {
-        const int own = decode_splits(n, n_kv, long_row);
+        const int64_t alone = part_bytes((int64_t)n * n_kv * G, decode_splits(n, n_kv, long_row, true), head_dim);
+        most = alone > most ? alone : most;
+        const int own = decode_splits(n, n_kv, long_row, false);
         const int shr = shared_splits(prefill_tiles(n, 1, G), n_kv, long_row, head_dim);
         const int64_t b = part_bytes((int64_t)n * n_kv * G, own + shr, head_dim);
         most = b > most ? b : most;
@@ -598,7 +648,7 @@ extern "C" int32_t locks_window_decode(
     if (n_req == 0) return 0;
     long keys = bound_keys(max_seq_len, bt_cols, page);
     if (window && (long)window + sinks + 32 < keys) keys = (long)window + sinks + 32;
-    const int ns = decode_splits(n_req, n_kv, keys);
+    const int ns = decode_splits(n_req, n_kv, keys, true);
     const int64_t rows = (int64_t)n_req * n_kv * G;
     rc = check_ws(what, workspace, workspace_bytes, part_bytes(rows, ns, head_dim));
     if (rc) return rc;
@@ -606,7 +656,7 @@ extern "C" int32_t locks_window_decode(
     const long ks[3] = {k_stride_block, k_stride_tok, k_stride_head}, vs[3] = {v_stride_block, v_stride_tok, v_stride_head};
     hipStream_t st = (hipStream_t)stream;
     rc = launch_decode_range(q, q_stride_req, q_stride_head, k_cache, ks, v_cache, vs, num_blocks, block_table, bt_stride,
-                             bt_cols, seq_lens, p, RangeSrc{window, sinks, nullptr, nullptr, 0, 0}, ns, 4, n_req, n_kv, G,
+                             bt_cols, seq_lens, p, RangeSrc{window, sinks}, ns, 4, n_req, n_kv, G,
                              head_dim, page, scale, st);
     if (rc) return rc;
     return launch_merge(p, out, out_stride_req, out_stride_head, lse, lse_stride_req, n_req, n_kv, G, head_dim, nullptr, 0, st);
@@ -651,7 +701,7 @@ extern "C" int32_t locks_window_prefill(
     const TileArgs a{q, q_stride_tok, q_stride_head, k_cache, k_stride_block, k_stride_tok, k_stride_head, v_cache,
                      v_stride_block, v_stride_tok, v_stride_head, block_table, bt_stride, seq_lens, query_start_loc, nullptr,
                      out, out_stride_tok, out_stride_head, lse, lse_stride_tok, p, scale * kLog2e, scale, num_blocks, bt_cols,
-                     n_tokens, n_req, n_kv, G, page == 16 ? 4 : page == 32 ? 5 : 6, window, sinks, ns};
+                     n_tokens, n_req, n_kv, G, page == 16 ? 4 : page == 32 ? 5 : 6, window, sinks, ns, 0, 0, 0, 1};
     hipStream_t st = (hipStream_t)stream;
     const dim3 grid((unsigned)(tiles * n_kv * ns));
     if (ns == 1) { AT_LAUNCH(false, false); return check_launch("attn_tile_kernel"); }
@@ -684,25 +734,21 @@ extern "C" int32_t locks_prefix_decode(
     const long keys = bound_keys(max_seq_len, bt_cols, page);
     const long pre = max_prefix_pages ? (long)max_prefix_pages * page : keys;
     const long tiles = prefill_tiles(n_req, n_groups, G);
-    const int own = decode_splits(n_req, n_kv, keys), shr = shared_splits(tiles, n_kv, pre < keys ? pre : keys, head_dim);
+    const int own = decode_splits(n_req, n_kv, keys, false), shr = shared_splits(tiles, n_kv, pre < keys ? pre : keys, head_dim);
     const int64_t rows = (int64_t)n_req * n_kv * G;
-    LOCKS_REQUIRE(tiles * n_kv * shr <= 0x7fffffffL, "%s: too many requests and heads for one launch", what);
+    LOCKS_REQUIRE((tiles * shr + (long)n_req * own) * n_kv <= 0x7fffffffL, "%s: too many requests and heads for one launch", what);
     rc = check_ws(what, workspace, workspace_bytes, part_bytes(rows, own + shr, head_dim));
     if (rc) return rc;
     const Partials p = layout(workspace, rows, own + shr, head_dim);
     const TileArgs a{q, q_stride_req, q_stride_head, k_cache, k_stride_block, k_stride_tok, k_stride_head, v_cache,
                      v_stride_block, v_stride_tok, v_stride_head, block_table, bt_stride, seq_lens, group_start, prefix_pages,
                      nullptr, 0, 0, nullptr, 0, p, scale * kLog2e, scale, num_blocks, bt_cols, n_req, n_groups, n_kv, G,
-                     page == 16 ? 4 : page == 32 ? 5 : 6, 0, 0, shr};
+                     page == 16 ? 4 : page == 32 ? 5 : 6, 0, 0, shr, own, (int)(tiles * shr), n_req * own,
+                     n_kv < 256 ? 256 / n_kv : 1};
     hipStream_t st = (hipStream_t)stream;
-    const dim3 grid((unsigned)(tiles * n_kv * shr));
+    const dim3 grid((unsigned)((tiles * shr + (long)n_req * own) * n_kv));
     AT_LAUNCH(true, true);
     rc = check_launch("attn_tile_kernel<shared>");
-    if (rc) return rc;
-    const long ks[3] = {k_stride_block, k_stride_tok, k_stride_head}, vs[3] = {v_stride_block, v_stride_tok, v_stride_head};
-    rc = launch_decode_range(q, q_stride_req, q_stride_head, k_cache, ks, v_cache, vs, num_blocks, block_table, bt_stride,
-                             bt_cols, seq_lens, p, RangeSrc{0, 0, group_start, prefix_pages, n_groups, shr}, own, 4, n_req,
-                             n_kv, G, head_dim, page, scale, st);
     if (rc) return rc;
     return launch_merge(p, out, out_stride_req, out_stride_head, lse, lse_stride_req, n_req, n_kv, G, head_dim, nullptr, 0, st);
 }
