@@ -3,6 +3,10 @@
 #include <hip/hip_runtime.h>
 #include <stdarg.h>
 #include <stdio.h>
+#include <string.h>
+
+#include <type_traits>
+#include <utility>
 
 #include "locks_hip.h"
 
@@ -31,3 +35,50 @@ int check_launch(const char* what) {
 extern "C" const char* locks_last_error(void) { return locks::g_err; }
 
 extern "C" int32_t locks_abi_version(void) { return LOCKS_ABI_VERSION; }
+
+// ---- entries called with their arguments as one array of 8-byte words --------
+namespace {
+
+template <typename T>
+T word_as(uint64_t w) {
+    if constexpr (std::is_same_v<T, float>) {
+        double d;
+        memcpy(&d, &w, sizeof(d));
+        return (float)d;
+    } else if constexpr (std::is_pointer_v<T>) {
+        return reinterpret_cast<T>(w);
+    } else {
+        static_assert(std::is_integral_v<T>, "an integer, a float or a pointer");
+        return static_cast<T>(w);
+    }
+}
+template <typename... A, size_t... I>
+int32_t call_with(int32_t (*entry)(A...), const uint64_t* w, std::index_sequence<I...>) {
+    return entry(word_as<A>(w[I])...);
+}
+template <typename... A>
+int32_t call_with(int32_t (*entry)(A...), const uint64_t* w, int32_t n) {
+    if (n != (int32_t)sizeof...(A)) {
+        locks::set_error("locks_call: %d words for an entry of %d arguments", n, (int)sizeof...(A));
+        return -1;
+    }
+    return call_with(entry, w, std::index_sequence_for<A...>{});
+}
+
+}  // namespace
+
+extern "C" int32_t locks_call(int32_t entry, const uint64_t* words, int32_t n) {
+    if (!words) {
+        locks::set_error("locks_call: null words");
+        return -1;
+    }
+    switch (entry) {
+        case LOCKS_CALL_TABLES_STEP: return call_with(locks_tables_step, words, n);
+        case LOCKS_CALL_TABLES_TRIM: return call_with(locks_tables_trim, words, n);
+        case LOCKS_CALL_QKV_WRITE: return call_with(locks_qkv_write, words, n);
+        case LOCKS_CALL_WINDOW_DECODE: return call_with(locks_window_decode, words, n);
+        case LOCKS_CALL_WINDOW_PREFILL: return call_with(locks_window_prefill, words, n);
+        case LOCKS_CALL_PREFIX_DECODE: return call_with(locks_prefix_decode, words, n);
+        default: locks::set_error("locks_call: no entry %d", entry); return -1;
+    }
+}

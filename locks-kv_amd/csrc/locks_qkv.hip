@@ -235,7 +235,7 @@ extern "C" int32_t locks_qkv_write(
     else hipLaunchKernelGGL((qkv_write_kernel<DV, ITV, false>), dim3(cdiv(a.groups, QK_WAVES * ITV), nt),     \
                             dim3(QK_BLK), 0, st, b)
         if (head_dim == 64) { LAUNCH(64, 1); }
-        else if (head_dim == 128) { LAUNCH(128, 1); }
+        else if (head_dim == 128) { LAUNCH(128, 3); }
         else { LAUNCH(256, 1); }
 #undef LAUNCH
         const int rc = check_launch("qkv_write_kernel");

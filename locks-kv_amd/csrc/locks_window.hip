@@ -520,6 +520,7 @@ __global__ __launch_bounds__(AT_BLK, D == 256 ? 1 : 2) void attn_tile_kernel(con
 // Joins the partials of a row's splits: one workgroup per (token, head), D / 4
 // columns of four x 1024 / D streams over the splits.
 constexpr int AM_BLK = 256;
+constexpr int AM_PF = 4;                    // partials that a thread loads ahead
 template <int D>
 __global__ __launch_bounds__(AM_BLK) void attn_merge_kernel(const Partials p, uint16_t* __restrict__ out, long o_st,
                                                             long o_sh, float* __restrict__ lse, long lse_st, int n_kv,
@@ -535,7 +536,14 @@ __global__ __launch_bounds__(AM_BLK) void attn_merge_kernel(const Partials p, ui
     // rows before the first request or after the last one have no partials
     if (starts && (t < starts[0] || t >= starts[n_seq])) return;
     const long row0 = (t * n_kv + hd / G) * p.splits * G + hd % G;     // of split 0; G apart
-    // each wave the same: up to two splits per lane
+    // Every load goes out before anything waits: up to two splits' m and l per lane
+    // (each wave the same), and this thread's first AM_PF partials, wanted or not (a
+    // split without keys has no acc: what is there is left out by a select).
+    const float* ap = p.acc + row0 * D + 4 * col;
+    float4 pre[AM_PF];
+#pragma unroll
+    for (int k = 0; k < AM_PF; ++k)
+        pre[k] = *reinterpret_cast<const float4*>(ap + (long)min(strm + k * STREAMS, p.splits - 1) * G * D);
     float ms[2], ls[2];
     float mm = -INFINITY;
 #pragma unroll
@@ -557,10 +565,18 @@ __global__ __launch_bounds__(AM_BLK) void attn_merge_kernel(const Partials p, ui
     lt = wave_sum(lt);
     __syncthreads();
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    const float* ap = p.acc + row0 * D + 4 * col;
-    for (int s = strm; s < p.splits; s += STREAMS) {
+#pragma unroll
+    for (int k = 0; k < AM_PF; ++k) {
+        const int s = strm + k * STREAMS;
+        const float w = s < p.splits ? w_s[s] : 0.f;
+        acc.x = w != 0.f ? acc.x + w * pre[k].x : acc.x;
+        acc.y = w != 0.f ? acc.y + w * pre[k].y : acc.y;
+        acc.z = w != 0.f ? acc.z + w * pre[k].z : acc.z;
+        acc.w = w != 0.f ? acc.w + w * pre[k].w : acc.w;
+    }
+    for (int s = strm + AM_PF * STREAMS; s < p.splits; s += STREAMS) {
         const float w = w_s[s];
-        if (w != 0.f) {                     // a split without keys has no acc
+        if (w != 0.f) {
             const float4 x = *reinterpret_cast<const float4*>(ap + (long)s * G * D);
             acc.x += w * x.x; acc.y += w * x.y; acc.z += w * x.z; acc.w += w * x.w;
         }

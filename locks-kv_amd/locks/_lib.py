@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 
 _LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_lib", "liblocks_hip.so")
 ABI_VERSION = 11
@@ -109,6 +110,7 @@ SIGNATURES = {
     "locks_prefix_decode": (_i32, [_p, _i64, _i64, _p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _i32, _p,
                                    _i64, _i32, _p, _p, _p, _i32, _p, _i64, _i64, _p, _i64, _p, _i64, _i32,
                                    _i32, _i32, _i32, _i32, _i32, _i32, _f32, _p]),
+    "locks_call": (_i32, [_i32, _p, _i32]),
     "locks_decode_merge": (_i32, [_p, _p, _p, _p, _i64, _i32, _p, _i64, _i64, _i32, _i32, _i32,
                                   _i32, _i32, _i32, _i32, _i32, _p]),
 }
@@ -164,17 +166,30 @@ def rows_arg(st) -> int:
     return 0 if rb is None else _c.addressof(rb)
 
 
-def launch(fn, what: str, index: int, args: tuple) -> None:
-    """fn(*args, stream) on device `index` and its current stream, whichever
-    device is the current one; raises where it refuses."""
+def _words(name: str) -> struct.Struct:
+    return struct.Struct("=" + "".join("d" if t is _f32 else "q" for t in SIGNATURES[name][1]))
+
+
+# entry -> (its number for locks_call, the packer of its arguments)
+_CALLS = {name: (i, _words(name)) for i, name in enumerate((
+    "locks_tables_step", "locks_tables_trim", "locks_qkv_write", "locks_window_decode", "locks_window_prefill",
+    "locks_prefix_decode"))}
+
+
+def launch(name: str, index: int, args: tuple) -> None:
+    """Entry `name` with (*args, stream) on device `index` and its current stream,
+    whichever device is the current one; raises where it refuses.  The arguments go
+    as one block of words (locks_call)."""
     import torch
+    entry, packer = _CALLS[name]
+    call = load().locks_call
     if index == torch._C._cuda_getDevice():
-        rc = fn(*args, stream_ptr(index))
+        rc = call(entry, packer.pack(*args, stream_ptr(index)), len(args) + 1)
     else:
         with torch.cuda.device(index):
-            rc = fn(*args, stream_ptr(index))
+            rc = call(entry, packer.pack(*args, stream_ptr(index)), len(args) + 1)
     if rc:
-        check(rc, what)
+        check(rc, name)
 
 
 def stream_ptr(device=None) -> int:

@@ -13,7 +13,7 @@ from .. import _lib
 from .decode import _kv_args
 
 
-_BF16, _F32 = torch.bfloat16, torch.float32
+_BF16, _F32, _I32, _I64 = torch.bfloat16, torch.float32, torch.int32, torch.int64
 
 
 def _rows(name: str, t, n: int, heads, d: int, device) -> None:
@@ -86,45 +86,59 @@ def qk_norm_rope_write(q, k, v, positions, slot_mapping, kv_cache, cos_sin, q_ou
     A slot outside the cache (padding: -1) writes no cache row.  A position
     outside the table writes none either, and NaN to the token's ``q_out`` and
     ``k_out`` rows.  Slots of one call are distinct."""
-    n = q.shape[0] if n_tokens is None else n_tokens
+    # one pass over the tensors' attributes, unpacked at once (slices of shapes and a
+    # message at each check took longer than the launch); _refuse has the messages
     index = kv_cache.get_device()
-    # one pass over the tensors' attributes; _refuse has the messages
-    cs, qs, ks_, vs_, os = kv_cache.shape, q.shape, k.shape, v.shape, q_out.shape
-    qt, kt, vt, ot = q.stride(), k.stride(), v.stride(), q_out.stride()
-    ok = (index >= 0 and len(cs) == 5 and kv_cache.dtype is _BF16 and q.dtype is _BF16 and k.dtype is _BF16
-          and v.dtype is _BF16 and q_out.dtype is _BF16 and positions.dtype is torch.int32
-          and slot_mapping.dtype is torch.int64 and len(qs) == 3 and len(ks_) == 3 and vs_[1:] == ks_[1:]
-          and os[1:] == qs[1:] and n >= 0 and qs[0] >= n and ks_[0] >= n and vs_[0] >= n and os[0] >= n
-          and ks_[1:] == cs[3:] and qs[2] == cs[4] and qt[2] == 1 and kt[2] == 1 and vt[2] == 1 and ot[2] == 1
-          and positions.dim() == 1 and positions.is_contiguous() and slot_mapping.dim() == 1
-          and slot_mapping.is_contiguous() and positions.shape[0] >= n and slot_mapping.shape[0] >= n
-          and q.get_device() == index and k.get_device() == index and v.get_device() == index
-          and q_out.get_device() == index and positions.get_device() == index and slot_mapping.get_device() == index)
-    rot, max_pos, cp, f32, ko = 0, 0x7FFFFFFF, 0, None, (0, 0, 0)
-    if ok and cos_sin is not None:
-        ok = (cos_sin.dtype is _F32 and cos_sin.dim() == 2 and cos_sin.is_contiguous() and cos_sin.get_device() == index)
-        cp = cos_sin.data_ptr()
-        if ok:
+    try:
+        n0, n1, page, n_kv, d = kv_cache.shape
+        tq, H, dq = q.shape
+        tk, hk, dk = k.shape
+        tv, hv, dv = v.shape
+        to, ho, do = q_out.shape
+        (tp,), (ts,) = positions.shape, slot_mapping.shape
+        c0, c1, cst, csh, c4 = kv_cache.stride()
+        (q0, q1, q2), (k0, k1, k2), (v0, v1, v2), (o0, o1, o2) = q.stride(), k.stride(), v.stride(), q_out.stride()
+        (ps,), (ss,) = positions.stride(), slot_mapping.stride()
+        rot, max_pos, cp, f32, qw, kw, ko, ko0, ko1 = 0, 0x7FFFFFFF, 0, None, 0, 0, 0, 0, 0
+        n = tq if n_tokens is None else n_tokens
+        # either cache layout: K and V halves by the first or the second dim
+        first = n0 == 2 and n1 != 2
+        NB = n1 if first else n0
+        ok = (index >= 0 and kv_cache.dtype is _BF16 and q.dtype is _BF16 and k.dtype is _BF16 and v.dtype is _BF16
+              and q_out.dtype is _BF16 and positions.dtype is _I32 and slot_mapping.dtype is _I64 and 0 <= n <= tq
+              and n <= tk and n <= tv and n <= to and n <= tp and n <= ts and hk == n_kv and hv == n_kv and ho == H
+              and dq == d and dk == d and dv == d and do == d and c4 == 1 and q2 == 1 and k2 == 1 and v2 == 1 and o2 == 1
+              and (ps == 1 or tp < 2) and (ss == 1 or ts < 2) and (first or n1 != 1) and q.get_device() == index
+              and k.get_device() == index and v.get_device() == index and q_out.get_device() == index
+              and positions.get_device() == index and slot_mapping.get_device() == index)
+        if ok and cos_sin is not None:
             max_pos, rot = cos_sin.shape
-    for w in (q_weight, k_weight):
-        if ok and w is not None:
-            t = w.dtype
-            ok = ((t is _BF16 or t is _F32) and (f32 is None or t is f32) and w.dim() == 1 and w.shape[0] == cs[4]
-                  and w.is_contiguous() and w.get_device() == index)
-            f32 = t
-    if ok and k_out is not None:
-        kos, kot = k_out.shape, k_out.stride()
-        ok = (k_out.dtype is _BF16 and len(kos) == 3 and kos[0] >= n and kos[1:] == ks_[1:] and kot[2] == 1
-              and k_out.get_device() == index)
-        ko = (k_out.data_ptr(), *kot[:2])
-    if ok:
-        kp, vp, ks, (NB, page, n_kv, d) = _kv_args(kv_cache)
-        ok = vp is not None and kv_cache.stride(4) == 1
+            ok = cos_sin.dtype is _F32 and cos_sin.is_contiguous() and cos_sin.get_device() == index
+            cp = cos_sin.data_ptr()
+        for w in (q_weight, k_weight):
+            if ok and w is not None:
+                (wd,), t = w.shape, w.dtype
+                ok = (wd == d and (t is _BF16 or t is _F32) and (f32 is None or t is f32) and w.is_contiguous()
+                      and w.get_device() == index)
+                f32 = t
+        if ok and k_out is not None:
+            (t0, t1, t2), (ko0, ko1, ko2) = k_out.shape, k_out.stride()
+            ok = (k_out.dtype is _BF16 and t0 >= n and t1 == n_kv and t2 == d and ko2 == 1
+                  and k_out.get_device() == index)
+            ko = k_out.data_ptr()
+    except ValueError:                                       # another number of dims
+        ok, n = False, q.shape[0] if n_tokens is None else n_tokens
     if not ok:
         _refuse(q, k, v, positions, slot_mapping, kv_cache, cos_sin, q_out, n, q_weight, k_weight, k_out)
     if n == 0:
         return
-    _lib.launch(_lib.load().locks_qkv_write, "qkv_write", index, (
-        q.data_ptr(), qt[0], qt[1], k.data_ptr(), kt[0], kt[1], v.data_ptr(), vt[0], vt[1], positions.data_ptr(),
-        slot_mapping.data_ptr(), kp, *ks, vp, *ks, NB, cp, max_pos, rot, 1 if interleaved else 0, _lib.ptr(q_weight),
-        _lib.ptr(k_weight), 1 if f32 is _F32 else 0, eps, q_out.data_ptr(), ot[0], ot[1], *ko, n, qs[1], n_kv, d, page))
+    kp = kv_cache.data_ptr()
+    cb = c1 if first else c0
+    if q_weight is not None:
+        qw = q_weight.data_ptr()
+    if k_weight is not None:
+        kw = k_weight.data_ptr()
+    _lib.launch("locks_qkv_write", index, (
+        q.data_ptr(), q0, q1, k.data_ptr(), k0, k1, v.data_ptr(), v0, v1, positions.data_ptr(), slot_mapping.data_ptr(),
+        kp, cb, cst, csh, kp + 2 * (c0 if first else c1), cb, cst, csh, NB, cp, max_pos, rot, 1 if interleaved else 0,
+        qw, kw, 1 if f32 is _F32 else 0, eps, q_out.data_ptr(), o0, o1, ko, ko0, ko1, n, H, n_kv, d, page))

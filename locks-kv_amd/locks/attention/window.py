@@ -76,29 +76,36 @@ def _args(what: str, q, kv_cache, block_table, seq_lens, out, ws, lse, rows: int
     arguments: of q up to seq_lens; from out to the workspace; n_kv, G, d, page; the
     device's index."""
     index = kv_cache.get_device()
-    qs, os, qt, ot, bs, bt = q.shape, out.shape, q.stride(), out.stride(), block_table.shape, block_table.stride()
-    ok = (index >= 0 and kv_cache.dim() == 5 and kv_cache.dtype is _BF16 and q.dtype is _BF16 and out.dtype is _BF16
-          and block_table.dtype is _I32 and seq_lens.dtype is _I32 and len(qs) == 3 and len(os) == 3 and len(bs) == 2
-          and qt[2] == 1 and ot[2] == 1 and bt[1] == 1 and seq_lens.dim() == 1 and seq_lens.is_contiguous()
-          and rows >= 0 and n_req >= 0 and qs[0] >= rows and os[0] >= rows and bs[0] >= n_req
-          and seq_lens.shape[0] >= n_req and q.get_device() == index and out.get_device() == index
-          and block_table.get_device() == index and seq_lens.get_device() == index
-          and (ws is None or (ws.get_device() == index and ws.is_contiguous())))
-    if ok:
-        kp, vp, ks, (NB, page, n_kv, d) = _kv_args(kv_cache)
-        H = qs[1]
-        ok = vp is not None and kv_cache.stride(4) == 1 and H % n_kv == 0 and os[1] == H and qs[2] == d and os[2] == d
-        lp = ls = 0
+    try:
+        n0, n1, page, n_kv, d = kv_cache.shape
+        c0, c1, cst, csh, c4 = kv_cache.stride()
+        (tq, H, dq), (to, ho, do), (rb, cols), (ts,) = q.shape, out.shape, block_table.shape, seq_lens.shape
+        (q0, q1, q2), (o0, o1, o2), (b0, b1), (ss,) = q.stride(), out.stride(), block_table.stride(), seq_lens.stride()
+        # either cache layout: K and V halves by the first or the second dim
+        first = n0 == 2 and n1 != 2
+        ok = (index >= 0 and kv_cache.dtype is _BF16 and q.dtype is _BF16 and out.dtype is _BF16
+              and block_table.dtype is _I32 and seq_lens.dtype is _I32 and 0 <= rows <= tq and rows <= to
+              and 0 <= n_req <= rb and n_req <= ts and H % n_kv == 0 and ho == H and dq == d and do == d and c4 == 1
+              and q2 == 1 and o2 == 1 and b1 == 1 and (ss == 1 or ts < 2) and (first or n1 != 1)
+              and q.get_device() == index and out.get_device() == index and block_table.get_device() == index
+              and seq_lens.get_device() == index)
+        lp = ls = wp = wb = 0
+        if ok and ws is not None:
+            ok = ws.get_device() == index and ws.is_contiguous()
+            wp, wb = ws.data_ptr(), ws.nbytes
         if ok and lse is not None:
-            zs, zt = lse.shape, lse.stride()
-            ok = (lse.dtype is _F32 and len(zs) == 2 and zt[1] == 1 and zs[0] >= rows and zs[1] == H
-                  and lse.get_device() == index)
-            lp, ls = lse.data_ptr(), zt[0]
+            (tl, hl), (ls, l1) = lse.shape, lse.stride()
+            ok = lse.dtype is _F32 and l1 == 1 and tl >= rows and hl == H and lse.get_device() == index
+            lp = lse.data_ptr()
+    except ValueError:                                       # another number of dims
+        ok = False
     if not ok:
         _refuse(what, q, kv_cache, block_table, seq_lens, out, ws, lse, rows, n_req)
-    head = (q.data_ptr(), qt[0], qt[1], kp, *ks, vp, *ks, NB, block_table.data_ptr(), bt[0], bs[1], seq_lens.data_ptr())
-    tail = (out.data_ptr(), ot[0], ot[1], lp, ls, *((0, 0) if ws is None else (ws.data_ptr(), ws.nbytes)))
-    return head, tail, (n_kv, H // n_kv, d, page), index
+    kp = kv_cache.data_ptr()
+    cb = c1 if first else c0
+    head = (q.data_ptr(), q0, q1, kp, cb, cst, csh, kp + 2 * (c0 if first else c1), cb, cst, csh, n1 if first else n0,
+            block_table.data_ptr(), b0, cols, seq_lens.data_ptr())
+    return head, (out.data_ptr(), o0, o1, lp, ls, wp, wb), (n_kv, H // n_kv, d, page), index
 
 
 def window_decode(q, kv_cache, block_table, seq_lens, out, ws, *, n_req: int, scale: float, window: int = 0,
@@ -112,7 +119,7 @@ def window_decode(q, kv_cache, block_table, seq_lens, out, ws, *, n_req: int, sc
     head, tail, geo, index = _args("window_decode", q, kv_cache, block_table, seq_lens, out, ws, lse, n_req, n_req)
     if n_req == 0:
         return
-    _lib.launch(_lib.load().locks_window_decode, "window_decode", index,
+    _lib.launch("locks_window_decode", index,
                 (*head, window, sinks, *tail, n_req, *geo, max_seq_len, scale))
 
 
@@ -128,7 +135,7 @@ def window_prefill(q, kv_cache, block_table, seq_lens, query_start_loc, out, ws,
     _i32("window_prefill: query_start_loc", query_start_loc, n_req + 1, index)
     if n_req == 0 or n_tokens == 0:
         return
-    _lib.launch(_lib.load().locks_window_prefill, "window_prefill", index,
+    _lib.launch("locks_window_prefill", index,
                 (*head, query_start_loc.data_ptr(), window, sinks, *tail, n_tokens, n_req, *geo, max_seq_len, scale))
 
 
@@ -145,6 +152,6 @@ def prefix_decode(q, kv_cache, block_table, seq_lens, group_start, prefix_pages,
     _i32("prefix_decode: prefix_pages", prefix_pages, n_groups, index)
     if n_req == 0:
         return
-    _lib.launch(_lib.load().locks_prefix_decode, "prefix_decode", index,
+    _lib.launch("locks_prefix_decode", index,
                 (*head, group_start.data_ptr(), prefix_pages.data_ptr(), n_groups, *tail, n_req, *geo, max_prefix_pages,
                  max_seq_len, scale))

@@ -111,7 +111,7 @@ class BlockTables:
             raise ValueError(f"n_req {n_req} outside [0, max_reqs {self.max_reqs}]")
         if not 0 <= n_tokens <= self.max_tokens:
             raise ValueError(f"n_tokens {n_tokens} outside [0, max_tokens {self.max_tokens}]")
-        _lib.launch(_lib.load().locks_tables_step, "tables_step", self._index, (
+        _lib.launch("locks_tables_step", self._index, (
             self._check("rows", rows, n_req), self._check("new_lens", new_lens, n_req), n_req, n_tokens, *self._step_args))
 
     def trim(self, rows, keep_lens, n_req: int) -> None:
@@ -127,5 +127,5 @@ class BlockTables:
         n_req = int(n_req)
         if not 0 <= n_req <= self.max_reqs:
             raise ValueError(f"n_req {n_req} outside [0, max_reqs {self.max_reqs}]")
-        _lib.launch(_lib.load().locks_tables_trim, "tables_trim", self._index, (
+        _lib.launch("locks_tables_trim", self._index, (
             self._check("rows", rows, n_req), self._check("keep_lens", keep_lens, n_req), n_req, *self._trim_args))
