@@ -13,7 +13,8 @@
 // row rotations and one permlane swap at most).  The partner of an adjacent pair
 // is in the lane, that of a half-split pair rot / 16 lanes away (its raw bf16
 // comes over with four permutes and is normed again here).  Bound by memory: every
-// row is read and written once.
+// row is read and written once.  8192 tokens of 32 + 16 heads of 128: 45.8 us warm (4.5
+// TB/s), 50-53 cold; one token 3-5 us.
 #include "locks_common.h"
 #include "locks_hip.h"
 

@@ -17,9 +17,14 @@
 //   O^T += V^T P^T: the keys of an MFMA step are numbered so that a lane's P
 //     values are the operand as they stand; V comes out of LDS transposed
 //     (ds_read_b64_tr_b16: 4 keys x 16 columns per 16 lanes).
-// K and V arrive by direct loads to LDS, one tile ahead.  16-byte chunks of a
-// row are permuted by the row on the way in (an exclusive or), which keeps the
-// reads of both operands free of bank conflicts.
+// K and V arrive by direct loads to LDS, one tile ahead (two at d 64 and 256).
+// 16-byte chunks of a row are permuted by the row on the way in (an exclusive or),
+// which keeps the reads of both operands free of bank conflicts.
+// 8192 tokens, 32 / 8 heads, d 128, causal: 556 us, 989 TFLOP/s, the matrix cores
+// 42-45 % busy; copies for timing: without the softmax 496, without K and V reads
+// from LDS too 440, without staging too 353.  64 keys a tile and 4 waves: 32 keys
+// with four tiles in LDS took 580, 8 waves on 256 rows 548 there but 163 for 139 at
+// d 64 and 96 for 77 on a prefix.
 //
 // Decode (one token): the split kernel of locks_decode.hip over a token range, or
 // (with a shared prefix) the tiles above, of which a request fills one column block.
@@ -104,10 +109,11 @@ __global__ __launch_bounds__(AT_BLK, D == 256 ? 1 : 2) void attn_tile_kernel(con
     // one array per tile: the compiler can tell the DMA of one from the reads of
     // another, and waits for neither
     constexpr int NST = GM::NST, TB = GM::TILEB;
-    __shared__ __attribute__((aligned(1024))) uint8_t k0[TB], k1[TB], k2[NST > 2 ? TB : 16], k3[NST > 3 ? TB : 16];
-    __shared__ __attribute__((aligned(1024))) uint8_t v0[TB], v1[TB], v2[NST > 2 ? TB : 16], v3[NST > 3 ? TB : 16];
-    auto kbuf = [&](auto i) __attribute__((always_inline)) { return i() == 0 ? k0 : i() == 1 ? k1 : i() == 2 ? k2 : k3; };
-    auto vbuf = [&](auto i) __attribute__((always_inline)) { return i() == 0 ? v0 : i() == 1 ? v1 : i() == 2 ? v2 : v3; };
+    __shared__ __attribute__((aligned(1024))) uint8_t k0[TB], k1[TB], k2[NST > 2 ? TB : 16];
+    __shared__ __attribute__((aligned(1024))) uint8_t v0[TB], v1[TB], v2[NST > 2 ? TB : 16];
+    static_assert(NST == 2 || NST == 3, "tiles in LDS");
+    auto kbuf = [&](auto i) __attribute__((always_inline)) { return i() == 0 ? k0 : i() == 1 ? k1 : k2; };
+    auto vbuf = [&](auto i) __attribute__((always_inline)) { return i() == 0 ? v0 : i() == 1 ? v1 : v2; };
     __shared__ int wlim[AT_WAVES][4];
     __shared__ int odd[2];                              // a value that is not finite is in the tile
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -146,9 +152,9 @@ __global__ __launch_bounds__(AT_BLK, D == 256 ? 1 : 2) void attn_tile_kernel(con
     for (int s0 = 0, done = 0; s0 < a.n_seq && seq < 0; s0 += kWave) {
         // (all loads together: a tile of few keys lives as long as its chain of them)
         const int s = min(s0 + lane, a.n_seq - 1);
-        const int at = a.starts[s], end = min(a.starts[s + 1], a.n_rows);
+        const int at = a.starts[s], end = a.starts[s + 1];
         const int len_s = SHARED ? max(a.gpages[s], 0) : a.seq_lens[s];
-        const int f = max(at, 0), n = s0 + lane < a.n_seq ? max(end - f, 0) : 0;
+        const int f = max(at, 0), n = s0 + lane < a.n_seq ? max(min(end, a.n_rows) - f, 0) : 0;
         const int nt = (n + TQ - 1) / TQ;
         const int inc = wave_incl_scan_i(nt);
         const unsigned long long hit = __ballot(done + inc > tile);
@@ -454,33 +460,26 @@ __global__ __launch_bounds__(AT_BLK, D == 256 ? 1 : 2) void attn_tile_kernel(con
     auto tile_step = [&](int n, auto use, auto fill) __attribute__((always_inline)) {
         const int behind = min(n1 - 1 - n, NST - 2);
         if (behind == 0) __builtin_amdgcn_s_waitcnt(vm_wait(0));
-        else if (behind == 1) __builtin_amdgcn_s_waitcnt(vm_wait(2 * GM::NI));
-        else __builtin_amdgcn_s_waitcnt(vm_wait(4 * GM::NI));
+        else __builtin_amdgcn_s_waitcnt(vm_wait(2 * GM::NI));
         lds_barrier();
         if (n + NST - 1 < n1) stage(n + NST - 1, kbuf(fill), vbuf(fill));
         compute(n, kbuf(use), vbuf(use));
     };
     using I0 = std::integral_constant<int, 0>; using I1 = std::integral_constant<int, 1>;
-    using I2 = std::integral_constant<int, 2>; using I3 = std::integral_constant<int, 3>;
+    using I2 = std::integral_constant<int, 2>;
     if (n0 < n1) {
         fetch_ids(n0);
         stage(n0, k0, v0);
         if constexpr (NST > 2) { if (n0 + 1 < n1) stage(n0 + 1, k1, v1); }
-        if constexpr (NST > 3) { if (n0 + 2 < n1) stage(n0 + 2, k2, v2); }
     }
     for (int n = n0; n < n1; n += NST) {
         if constexpr (NST == 2) {
             tile_step(n, I0{}, I1{});
             if (n + 1 < n1) tile_step(n + 1, I1{}, I0{});
-        } else if constexpr (NST == 3) {
+        } else {
             tile_step(n, I0{}, I2{});
             if (n + 1 < n1) tile_step(n + 1, I1{}, I0{});
             if (n + 2 < n1) tile_step(n + 2, I2{}, I1{});
-        } else {
-            tile_step(n, I0{}, I3{});
-            if (n + 1 < n1) tile_step(n + 1, I1{}, I0{});
-            if (n + 2 < n1) tile_step(n + 2, I2{}, I1{});
-            if (n + 3 < n1) tile_step(n + 3, I3{}, I2{});
         }
     }
 
@@ -518,7 +517,9 @@ __global__ __launch_bounds__(AT_BLK, D == 256 ? 1 : 2) void attn_tile_kernel(con
 }
 
 // Joins the partials of a row's splits: one workgroup per (token, head), D / 4
-// columns of four x 1024 / D streams over the splits.
+// columns of four x 1024 / D streams over the splits.  Bound by its chain of loads
+// for few rows (32 heads of 33 splits 4.0 us), by memory for many (2048 heads of 17
+// splits 6.3 us, 2.8 TB/s).
 constexpr int AM_BLK = 256;
 constexpr int AM_PF = 4;                    // partials that a thread loads ahead
 template <int D>
@@ -604,10 +605,11 @@ static int clampi(long x, int lo, int hi) { return (int)(x < lo ? lo : x > hi ? 
 // A single-token call: about 512 workgroups (two per CU), each of at least 8
 // 16-token steps (two per wave).  With `even`, a row's splits hold at most 64 steps:
 // lengths differ, and the longest split is the call's time (32 ragged requests of a
-// window of 8192: 119 us at 2 splits, 96.5 at 9, 103 at 17).
+// window of 8192: 119 us at 2 splits, 96.5 at 9, 103 at 17), up to 4096 workgroups.
 static int decode_splits(int n_req, int n_kv, long max_keys, bool even) {
     const long rows = (long)n_req * n_kv, steps = (max_keys + 15) / 16;
-    const long fill = (512 + rows - 1) / rows, most = even ? (steps + 63) / 64 : 1;
+    const long fill = (512 + rows - 1) / rows, cap = (4096 + rows - 1) / rows;
+    const long most = !even ? 1 : (steps + 63) / 64 < cap ? (steps + 63) / 64 : cap;
     return clampi(fill > most ? fill : most, 1, clampi((steps + 7) / 8, 1, 64));
 }
 // Tiles of k non-empty requests (groups) of n tokens together: sum of ceil(c / TQ)

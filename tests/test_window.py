@@ -352,6 +352,20 @@ def test_other_stream_and_short_batches():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("lens, new", [([90, 70], [40, 30]), ([6000, 5000], [3, 2])])
+def test_fewer_rows_than_the_starts_say(lens, new):
+    """n_tokens inside the second request: its first rows keep their positions, the
+    others stay as they were."""
+    c = _case(lens, new, 2, 4, 128, 16)
+    n = new[0] + 1
+    out, lse = _outs(c)
+    window_prefill(c["q"], c["kv"], c["bt"], c["sl"], c["qsl"], out, _ws(c), n_req=2, n_tokens=n, window=33, sinks=2,
+                   scale=c["scale"], lse=lse)
+    _agree(out[:n], lse[:n], _exact(c, 33, 2), rows=n)
+    assert bool((out[n:] == 7).all()) and bool((lse[n:] == 7).all())
+
+
+@pytest.mark.gpu
 def test_large_scores_and_wide_values():
     """Scores of hundreds (one key takes all) and V past fp16's range."""
     c = _case([300], [1], 1, 4, 128, 16)
@@ -433,3 +447,6 @@ def test_workspace_covers_every_call():
     for n_kv, G, d in ((8, 4, 128), (1, 16, 64), (2, 3, 256)):
         b = [lib.locks_attn_workspace_bytes(n, n, n_kv, G, d) for n in (1, 2, 7, 64, 65, 300, 5000)]
         assert b == sorted(b) and b[0] > 0
+    # about 4096 workgroups' partials at most, past that one per row
+    assert lib.locks_attn_workspace_bytes(256, 8192, 8, 4, 128) < 1 << 28
+    assert lib.locks_attn_workspace_bytes(8192, 8192, 8, 4, 128) < 1 << 29
