@@ -13,8 +13,8 @@
 // row rotations and one permlane swap at most).  The partner of an adjacent pair
 // is in the lane, that of a half-split pair rot / 16 lanes away (its raw bf16
 // comes over with four permutes and is normed again here).  Bound by memory: every
-// row is read and written once.  8192 tokens of 32 + 16 heads of 128: 45.8 us warm (4.5
-// TB/s), 50-53 cold; one token 3-5 us.
+// row is read and written once.  8192 tokens of 32 + 16 heads of 128: 41 us, 5.0 TB/s,
+// a copy's rate; one token 3.8 us.
 #include "locks_common.h"
 #include "locks_hip.h"
 
@@ -35,7 +35,7 @@ struct QkvArgs {
     uint16_t* qo; long qo_st, qo_sh;
     uint16_t* ko; long ko_st, ko_sh;
     long slots;                             // num_blocks * page
-    int max_pos, rot, w_f32, n_tok, H, n_kv, pg_sh, groups;
+    int max_pos, rot, n_tok, H, n_kv, pg_sh, groups;
     float eps;
 };
 
@@ -44,22 +44,31 @@ __device__ __forceinline__ void unpack8(const uint4& w, float* x) {
     x[4] = bf16lo(w.z); x[5] = bf16hi(w.z); x[6] = bf16lo(w.w); x[7] = bf16hi(w.w);
 }
 __device__ __forceinline__ uint4 pack8(const float* x) {
-    uint4 w;
-    w.x = (uint32_t)f32_to_bf16(x[0]) | (uint32_t)f32_to_bf16(x[1]) << 16;
-    w.y = (uint32_t)f32_to_bf16(x[2]) | (uint32_t)f32_to_bf16(x[3]) << 16;
-    w.z = (uint32_t)f32_to_bf16(x[4]) | (uint32_t)f32_to_bf16(x[5]) << 16;
-    w.w = (uint32_t)f32_to_bf16(x[6]) | (uint32_t)f32_to_bf16(x[7]) << 16;
-    return w;
+    typedef __bf16 v8 __attribute__((ext_vector_type(8)));
+    v8 y;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = (__bf16)x[e];        // to nearest even, NaN kept
+    return __builtin_bit_cast(uint4, y);
 }
-__device__ __forceinline__ void load_weight(const void* w, int f32, int e0, float* x) {
-    if (f32) {
-        const float4 a = *reinterpret_cast<const float4*>(static_cast<const float*>(w) + e0);
-        const float4 b = *reinterpret_cast<const float4*>(static_cast<const float*>(w) + e0 + 4);
-        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-    } else {
-        unpack8(*reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(w) + e0), x);
+// Eight consecutive weights, as they stand in memory (bf16 or fp32).
+template <bool F32>
+struct Weights8 {
+    uint4 a, b;
+    __device__ __forceinline__ void load(const void* w, int e0) {
+        const uint4* p = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(w) + (F32 ? 4 : 2) * e0);
+        a = p[0];
+        if constexpr (F32) b = p[1];
     }
-}
+    __device__ __forceinline__ void get(float* x) const {
+        if constexpr (F32) {
+            const uint32_t u[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = __uint_as_float(u[e]);
+        } else {
+            unpack8(a, x);
+        }
+    }
+};
 
 // Sum over the D / 8 lanes of a head.
 template <int D>
@@ -75,7 +84,7 @@ __device__ __forceinline__ float head_sum(float s) {
     return s;
 }
 
-template <int D, int IT, bool INTER>
+template <int D, int IT, bool INTER, bool WF32>
 __global__ __launch_bounds__(QK_BLK) void qkv_write_kernel(const QkvArgs a)
 {
     constexpr int LPH = D / 8, HPW = kWave / LPH;       // lanes per head, heads per wave
@@ -98,7 +107,10 @@ __global__ __launch_bounds__(QK_BLK) void qkv_write_kernel(const QkvArgs a)
         const uint16_t* p = x < a.H ? a.q + (long)t * a.q_st + (long)x * a.q_sh
                           : x < a.H + a.n_kv ? a.k + (long)t * a.k_st + (long)(x - a.H) * a.k_sh
                                              : a.v + (long)t * a.v_st + (long)(x - a.H - a.n_kv) * a.v_sh;
-        raw[i] = *reinterpret_cast<const uint4*>(p + e0);
+        // read once: not kept in the caches, where the outputs' next reader finds them
+        // (8192 tokens 47.5 -> 45 us, with the attention behind it 133 -> 129; stores
+        // past the caches too: 42.5 alone, but 134 with the attention)
+        raw[i] = __builtin_bit_cast(uint4, __builtin_nontemporal_load(reinterpret_cast<const v4i*>(p + e0)));
     }
     const int pos = a.pos[t];
     const long slot = a.slot[t];
@@ -121,6 +133,11 @@ __global__ __launch_bounds__(QK_BLK) void qkv_write_kernel(const QkvArgs a)
             s[e] = y.x; s[e + 1] = y.y; s[e + 2] = y.z; s[e + 3] = y.w;
         }
     }
+    // weights of this lane's entries and of its partner's, for q and for k
+    Weights8<WF32> wq{}, wk{}, pq{}, pk{};
+    const int ep = !INTER && turned ? (low ? e0 + half : e0 - half) : e0;
+    if (a.qw) { wq.load(a.qw, e0); pq.load(a.qw, ep); }
+    if (a.kw) { wk.load(a.kw, e0); pk.load(a.kw, ep); }
     const long blk = slot >> a.pg_sh;
     const int off = (int)(slot & ((1 << a.pg_sh) - 1));
     const bool cached = placed && slot >= 0 && slot < a.slots;
@@ -128,7 +145,7 @@ __global__ __launch_bounds__(QK_BLK) void qkv_write_kernel(const QkvArgs a)
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
         const bool is_q = u[i] < a.H, is_k = !is_q && u[i] < a.H + a.n_kv;
-        const void* w = is_q ? a.qw : is_k ? a.kw : nullptr;
+        const bool normed = is_q ? a.qw != nullptr : is_k && a.kw != nullptr;
         float x[8], y[8];
         unpack8(raw[i], x);
         uint4 pr = raw[i];
@@ -141,16 +158,16 @@ __global__ __launch_bounds__(QK_BLK) void qkv_write_kernel(const QkvArgs a)
         for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
         ss = head_sum<D>(ss);
         unpack8(pr, y);
-        if (w) {
+        if (normed) {
             const float inv = rsqrtf(ss * (1.f / D) + a.eps);
-            float g[8];
-            load_weight(w, a.w_f32, e0, g);
+            float gq[8], gk[8];
+            wq.get(gq); wk.get(gk);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = x[e] * inv * g[e];
-            if (!INTER && turned) {
-                load_weight(w, a.w_f32, low ? e0 + half : e0 - half, g);
+            for (int e = 0; e < 8; ++e) x[e] = x[e] * inv * (is_q ? gq[e] : gk[e]);
+            if constexpr (!INTER) {
+                pq.get(gq); pk.get(gk);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) y[e] = y[e] * inv * g[e];
+                for (int e = 0; e < 8; ++e) y[e] = y[e] * inv * (is_q ? gq[e] : gk[e]);
             }
         }
         if (turned && (is_q || is_k)) {
@@ -219,21 +236,25 @@ extern "C" int32_t locks_qkv_write(
               positions, slot_mapping, k_cache, kc_stride_block, kc_stride_tok, kc_stride_head, v_cache,
               vc_stride_block, vc_stride_tok, vc_stride_head, cos_sin, q_weight, k_weight, q_out, qo_stride_tok,
               qo_stride_head, k_out, ko_stride_tok, ko_stride_head, (long)num_blocks * page, max_pos, rot,
-              weights_f32, n_tokens, n_heads, n_kv, page == 16 ? 4 : page == 32 ? 5 : 6,
+              n_tokens, n_heads, n_kv, page == 16 ? 4 : page == 32 ? 5 : 6,
               cdiv(n_heads + 2 * n_kv, per_wave), eps};
     hipStream_t st = (hipStream_t)stream;
     // groups per wave: the angles and weights of a token are loaded once for them,
-    // and their rows are in flight together (8192 tokens of 48 heads: 1 group 56 us,
-    // 3 groups 50)
+    // and their rows are in flight together (8192 tokens of 48 heads: 2 groups 50.5
+    // us, 3 and 4 45)
     constexpr int IT = 3;
     const long waves = (long)n_tokens * cdiv(a.groups, IT);
     const dim3 grid((unsigned)((waves + QK_WAVES - 1) / QK_WAVES));
-#define LAUNCH(DV)                                                                                           \
-    if (interleaved) hipLaunchKernelGGL((qkv_write_kernel<DV, IT, true>), grid, dim3(QK_BLK), 0, st, a);     \
-    else hipLaunchKernelGGL((qkv_write_kernel<DV, IT, false>), grid, dim3(QK_BLK), 0, st, a)
+#define LAUNCH_W(DV, INTER)                                                                                     \
+    if (weights_f32) hipLaunchKernelGGL((qkv_write_kernel<DV, IT, INTER, true>), grid, dim3(QK_BLK), 0, st, a); \
+    else hipLaunchKernelGGL((qkv_write_kernel<DV, IT, INTER, false>), grid, dim3(QK_BLK), 0, st, a)
+#define LAUNCH(DV)                              \
+    if (interleaved) { LAUNCH_W(DV, true); }    \
+    else { LAUNCH_W(DV, false); }
     if (head_dim == 64) { LAUNCH(64); }
     else if (head_dim == 128) { LAUNCH(128); }
     else { LAUNCH(256); }
 #undef LAUNCH
+#undef LAUNCH_W
     return check_launch("qkv_write_kernel");
 }

@@ -7,8 +7,10 @@ Layout:
     config.py            LocksConfig
     _lib.py              ctypes binding of liblocks_hip.so (HIP kernels)
     selection/           Rki4State, summary build, scorer, page selection
-    attention/           split-K sparse paged decode + LSE merge
-    backend/             plugin registration and the per-layer hot-path glue
+    attention/           split-K sparse paged decode + LSE merge; norm, rotation and
+                         cache write; window, prompt and shared-prefix attention
+    backend/             plugin registration, the per-layer hot-path glue, the
+                         engine-neutral driver and its block tables
 """
 from __future__ import annotations
 
