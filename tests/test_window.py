@@ -352,6 +352,16 @@ def test_other_stream_and_short_batches():
 
 
 @pytest.mark.gpu
+def test_many_requests():
+    """More requests than lanes, from none to a few tiles of new tokens each."""
+    new = [(r * 37) % 90 if r % 5 else 0 for r in range(150)]
+    lens = [n + (r * 53) % 200 for r, n in enumerate(new)]
+    c = _case(lens, new, 2, 4, 64, 16)
+    for window, sinks in ((0, 0), (60, 9)):
+        _agree(*_prefill(c, window, sinks), _exact(c, window, sinks))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("lens, new", [([90, 70], [40, 30]), ([6000, 5000], [3, 2])])
 def test_fewer_rows_than_the_starts_say(lens, new):
     """n_tokens inside the second request: its first rows keep their positions, the
