@@ -715,6 +715,7 @@ int32_t locks_qkv_write(const uint16_t* q, int64_t q_stride_tok, int64_t q_strid
  *   q, out (rows, n_kv * G, head_dim) bf16, element strides of (row, head);
  *   lse (rows, n_kv * G) f32 with row stride, or NULL: natural log of the sum
  *   of exp(scale * q.k) over the visible keys; K / V as for locks_decode_splitk
+ *   with token strides in [0, 2^24) elements, q, K and V 16-byte aligned
  *   block_table (n_req, bt_cols) i32: block ids are clamped to [0, num_blocks)
  *   seq_lens (n_req,) i32, this step's tokens included; a length past bt_cols *
  *   page sees only the table's tokens
