@@ -767,8 +767,10 @@ int32_t locks_window_prefill(const uint16_t* q, int64_t q_stride_tok, int64_t q_
 /* One query per request over all its keys, where the requests [group_start[g],
  * group_start[g + 1]) (group_start (n_groups + 1,) ascending) share their first
  * prefix_pages[g] pages: these are read once for the group, through the block
- * table row of its first request.  A member shorter than the prefix sees only its
- * own length.  A request in no group is attended like any other.
+ * table row of a member that is as long as the prefix (of its longest one where
+ * none is); the rows of shorter members and of padding may hold anything past
+ * their own pages.  A member shorter than the prefix sees only its own length.  A
+ * request in no group is attended like any other.
  *   max_prefix_pages  host-side upper bound of prefix_pages (0: none); only sizes
  *                     the launch */
 int32_t locks_prefix_decode(const uint16_t* q, int64_t q_stride_req, int64_t q_stride_head,

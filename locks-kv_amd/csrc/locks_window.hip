@@ -195,6 +195,21 @@ __global__ __launch_bounds__(AT_BLK, D == 256 ? 1 : 2) void attn_tile_kernel(con
                 }
         }
         bt_row = first;
+        if (!own) {
+            // The prefix's page ids: the row of the longest of the first 64 members (of
+            // the next 64, and so on, until one is as long as the prefix).  A row that
+            // ends sooner holds fewer pages, that of an unserved request an earlier
+            // batch's.  No member sees further than the longest one's row.
+            int best = 0, who = 0;
+            for (int s0 = 0; s0 < count; s0 += kWave) {
+                const int i = s0 + lane, sl_i = i < count ? a.seq_lens[first + i] : 0;
+                who = sl_i > best ? i : who;
+                best = max(best, sl_i);
+                if (__any(best >= pre)) break;
+            }
+            const int top = wave_max_int(best);
+            bt_row += __builtin_amdgcn_readfirstlane(wave_min_int(best == top ? who : count - 1));
+        }
     } else {
         const int pos = len + j;
         hi = (int)min((long)pos + 1, cap);

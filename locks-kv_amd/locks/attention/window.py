@@ -144,9 +144,10 @@ def prefix_decode(q, kv_cache, block_table, seq_lens, group_start, prefix_pages,
     """``window_decode`` without a window for requests that share pages: requests
     ``group_start[g] .. group_start[g + 1]`` (ascending) hold the same ids in their
     first ``prefix_pages[g]`` columns, which are read once for the group, through
-    the row of its first request.  Both are int32 on the GPU, so that a captured
-    call follows them.  Requests outside all groups, members shorter than the
-    prefix and padding (length 0) are attended like any other."""
+    the row of a member that is as long (of the longest where none is).  Both are
+    int32 on the GPU, so that a captured call follows them.  Requests outside all
+    groups, members shorter than the prefix and padding (length 0) are attended
+    like any other; their rows need hold no more pages than their lengths."""
     head, tail, geo, index = _args("prefix_decode", q, kv_cache, block_table, seq_lens, out, ws, lse, n_req, n_req)
     _i32("prefix_decode: group_start", group_start, n_groups + 1, index)
     _i32("prefix_decode: prefix_pages", prefix_pages, n_groups, index)
