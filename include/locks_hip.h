@@ -787,9 +787,9 @@ int32_t locks_prefix_decode(const uint16_t* q, int64_t q_stride_req, int64_t q_s
                             void* stream);
 
 /* The entries of a serving step with their arguments as n 8-byte words in order
- * (integers and pointers as they are, floats as doubles): for bindings where every
- * argument of a foreign call costs (a ctypes call of 40 arguments 3.8 us, of words
- * packed at once 1.1 us). */
+ * (integers and pointers as they are, floats as doubles; an integer past its
+ * argument's 32 bits is refused): for bindings where every argument of a foreign
+ * call costs (a ctypes call of 40 arguments 3.8 us, of words packed at once 1.1). */
 #define LOCKS_CALL_TABLES_STEP 0
 #define LOCKS_CALL_TABLES_TRIM 1
 #define LOCKS_CALL_QKV_WRITE 2

@@ -39,6 +39,14 @@ extern "C" int32_t locks_abi_version(void) { return LOCKS_ABI_VERSION; }
 // ---- entries called with their arguments as one array of 8-byte words --------
 namespace {
 
+// An integer word that its argument's type does not hold is refused: cut to 32 bits
+// it would be another, good-looking value.
+template <typename T>
+bool word_fits(uint64_t w) {
+    if constexpr (std::is_integral_v<T>) return static_cast<int64_t>(w) == static_cast<int64_t>(static_cast<T>(w));
+    else return true;
+}
+
 template <typename T>
 T word_as(uint64_t w) {
     if constexpr (std::is_same_v<T, float>) {
@@ -54,6 +62,12 @@ T word_as(uint64_t w) {
 }
 template <typename... A, size_t... I>
 int32_t call_with(int32_t (*entry)(A...), const uint64_t* w, std::index_sequence<I...>) {
+    const bool fits[] = {word_fits<A>(w[I])...};
+    for (size_t i = 0; i < sizeof...(A); ++i)
+        if (!fits[i]) {
+            locks::set_error("locks_call: word %d is %lld, its argument has 32 bits", (int)i, (long long)w[i]);
+            return -1;
+        }
     return entry(word_as<A>(w[I])...);
 }
 template <typename... A>
