@@ -648,8 +648,8 @@ int32_t locks_mla_decode_dense(const uint16_t* q, int64_t q_stride_req, int64_t 
  * lens (max_reqs,) tokens of every row; free_list (num_blocks,), whose entries
  * [head, num_blocks) are free, the next one first; state (4,) i32: head, the
  * unserved requests of the last step, an arrival count (0 between calls).
- * Batch entry r is row rows[r] (-1: padding) with new_lens[r] new tokens;
- * it takes ceil((lens + new) / page) - ceil(lens / page) blocks, in batch
+ * Batch entry r is row rows[r] (-1: padding, which takes no token) with
+ * new_lens[r] new tokens; it takes ceil((lens + new) / page) - ceil(lens / page) blocks, in batch
  * order.  A request is served when they are there, its pages are at most
  * max_pages, and its row exists and is named for the first time; else it
  * changes nothing, its seq_len is 0 and its slots are -1.
@@ -735,8 +735,8 @@ int32_t locks_qkv_write(const uint16_t* q, int64_t q_stride_tok, int64_t q_strid
 int64_t locks_attn_workspace_bytes(int32_t max_reqs, int32_t max_tokens, int32_t n_kv, int32_t G,
                                    int32_t head_dim);
 
-/* One query per request at position seq_len - 1: keys [max(seq_len - window, 0),
- * seq_len) and [0, sinks); window 0: all keys. */
+/* One query per request, in row r for request r, at position seq_len - 1: keys
+ * [max(seq_len - window, 0), seq_len) and [0, sinks); window 0: all keys. */
 int32_t locks_window_decode(const uint16_t* q, int64_t q_stride_req, int64_t q_stride_head,
                             const uint16_t* k_cache, int64_t k_stride_block, int64_t k_stride_tok,
                             int64_t k_stride_head, const uint16_t* v_cache, int64_t v_stride_block,
@@ -764,7 +764,7 @@ int32_t locks_window_prefill(const uint16_t* q, int64_t q_stride_tok, int64_t q_
                              int32_t n_req, int32_t n_kv, int32_t G, int32_t head_dim, int32_t page,
                              int32_t max_seq_len, float scale, void* stream);
 
-/* One query per request over all its keys, where the requests [group_start[g],
+/* One query per request (row r) over all its keys, where the requests [group_start[g],
  * group_start[g + 1]) (group_start (n_groups + 1,) ascending) share their first
  * prefix_pages[g] pages: these are read once for the group, through the block
  * table row of a member that is as long as the prefix (of its longest one where

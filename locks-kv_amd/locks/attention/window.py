@@ -113,8 +113,10 @@ def window_decode(q, kv_cache, block_table, seq_lens, out, ws, *, n_req: int, sc
     """One new token per request, at position ``seq_lens - 1``: ``out[:n_req]``
     (T, H, d) bf16 = softmax attention of ``q`` over the keys of the last
     ``window`` positions, its own included, and of the first ``sinks`` (window 0:
-    all), and ``lse[:n_req]`` (T, H) fp32 the log-sum-exp of the scores.  A request
-    of length 0 (padding) gives zeros and -inf.  ``max_seq_len``: an upper bound of
+    all), and ``lse[:n_req]`` (T, H) fp32 the log-sum-exp of the scores.  Request r
+    reads and writes row r: padding takes a row here, though no token in
+    ``BlockTables.step``, and so stands behind the requests.  A request of length 0
+    (padding) gives zeros and -inf.  ``max_seq_len``: an upper bound of
     the lengths, where one is known, sizes the launch.  ``ws``: attn_workspace."""
     head, tail, geo, index = _args("window_decode", q, kv_cache, block_table, seq_lens, out, ws, lse, n_req, n_req)
     if n_req == 0:

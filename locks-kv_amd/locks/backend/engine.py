@@ -160,9 +160,10 @@ class LocksEngine:
                       lse=None) -> None:
         """One layer of any step with attention over the whole row, or over the
         last ``window`` tokens and the first ``sinks``, read from the paged cache.
-        The first ``n_decode`` requests have one new token each (default: all,
-        without ``query_start_loc``; none with it), the others the rows that
-        ``query_start_loc`` gives."""
+        The first ``n_decode`` requests have one new token each, in rows 0 to
+        ``n_decode`` - 1 (default: all, without ``query_start_loc``; none with it),
+        the others the rows that ``query_start_loc`` gives.  Padding takes no
+        token: it stands behind the requests with one, or after ``n_decode``."""
         if n_decode is None:
             n_decode = n_req if query_start_loc is None else 0
         if not 0 <= n_decode <= n_req or (n_decode < n_req and query_start_loc is None):
@@ -179,6 +180,7 @@ class LocksEngine:
     def forward_prefix(self, q, kv_cache, block_table, seq_lens, group_start, prefix_pages, n_req: int, n_groups: int,
                        scale: float, out, *, max_prefix_pages: int = 0, lse=None) -> None:
         """One layer of a single-token step over the whole rows of requests that
-        share their first pages (``prefix_decode``)."""
+        share their first pages (``prefix_decode``); request r is row r of ``q``,
+        padding behind the requests."""
         prefix_decode(q, kv_cache, block_table, seq_lens, group_start, prefix_pages, out, self._ws(), n_req=n_req,
                       n_groups=n_groups, scale=scale, max_prefix_pages=max_prefix_pages, lse=lse)

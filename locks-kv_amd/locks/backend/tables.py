@@ -31,7 +31,8 @@ class BlockTables:
     State: ``table`` (max_reqs, max_pages) page ids and ``lens`` (max_reqs,)
     tokens of every row; ``free`` (num_blocks,) whose entries [head, num_blocks)
     are the free blocks, the next one first; ``state`` (4,): head, the last
-    step's unserved requests, and a count that every call leaves at zero.  ``reserved`` blocks, the lowest ids, are never handed out.
+    step's unserved requests, and a count that every call leaves at zero.
+    ``reserved`` blocks, the lowest ids, are never handed out.
 
     Outputs of ``step``: ``block_table`` (max_reqs, max_pages), ``seq_lens``
     (max_reqs,), ``query_start_loc`` (max_reqs + 1,), ``positions`` (max_tokens,)
@@ -105,7 +106,13 @@ class BlockTables:
         such requests).  Padding requests have ``seq_lens`` 0, tokens past the
         last request position 0 and slot -1.  Entries of ``block_table`` past a
         request's pages, and of all outputs past ``n_req`` and ``n_tokens``, stay
-        as they were."""
+        as they were.
+
+        Padding (whatever its ``new_lens``) and requests without a new token take
+        no row of the step's tokens, an unserved request keeps its own.  Calls
+        that read row r for request r (``window_decode``, ``prefix_decode``, the
+        selected decode) therefore need padding and such requests behind all
+        others; calls that take ``query_start_loc`` find every request's rows."""
         n_req, n_tokens = int(n_req), int(n_tokens)
         if not 0 <= n_req <= self.max_reqs:
             raise ValueError(f"n_req {n_req} outside [0, max_reqs {self.max_reqs}]")
