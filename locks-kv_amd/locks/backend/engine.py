@@ -142,7 +142,7 @@ class LocksEngine:
         n = int(q.shape[0] if n_tokens is None else n_tokens)
         qk_norm_rope_write(q, k, v, positions, slot_mapping, self.kv_caches[layer], cos_sin, q_out, n_tokens=n,
                            q_weight=q_weight, k_weight=k_weight, eps=eps, interleaved=interleaved, k_out=self._k_out)
-        if self.tier is not None:
+        if self.tier is not None and n:
             self.write_kv(layer, self._k_out[:n], v[:n])
 
     def _ws(self):
