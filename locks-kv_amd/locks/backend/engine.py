@@ -79,7 +79,9 @@ class LocksEngine:
                 cfg, num_layers=len(self.kv_caches), num_blocks=int(K0.shape[0]),
                 n_kv=int(num_heads_kv), page=page, d=int(head_dim), max_reqs=int(max_num_seqs),
                 max_pages=self.st.max_pages, max_tokens=int(max_num_batched_tokens), device=dev)
-            self._k_out = torch.empty(self.max_tokens, int(num_heads_kv), int(head_dim), dtype=torch.bfloat16, device=dev)
+            if self.tier.offload_k:                  # the keys as cached, for the tier
+                self._k_out = torch.empty(self.max_tokens, int(num_heads_kv), int(head_dim), dtype=torch.bfloat16,
+                                          device=dev)
 
     @torch.no_grad()
     def prologue(self, block_table, seq_lens, query_start_loc, n_req: int,
@@ -138,12 +140,16 @@ class LocksEngine:
                   q_weight=None, k_weight=None, eps: float = 1e-6, interleaved: bool = False) -> None:
         """A layer's projection made ready (``qk_norm_rope_write``): queries to
         ``q_out``, keys and values to the layer's cache and, for the mem variants,
-        to the tier's staging pool (``write_kv``)."""
+        V (mem-kv: and the keys) to the tier's staging pool (``write_kv``).  This
+        and the dense calls need a cache with both halves: a K-only one, which the
+        mem variants' ``forward`` takes too, is refused."""
         n = int(q.shape[0] if n_tokens is None else n_tokens)
+        if self.tier is not None and n > self.max_tokens:
+            raise ValueError(f"write_qkv: {n} tokens > max_num_batched_tokens {self.max_tokens}")
         qk_norm_rope_write(q, k, v, positions, slot_mapping, self.kv_caches[layer], cos_sin, q_out, n_tokens=n,
                            q_weight=q_weight, k_weight=k_weight, eps=eps, interleaved=interleaved, k_out=self._k_out)
         if self.tier is not None and n:
-            self.write_kv(layer, self._k_out[:n], v[:n])
+            self.write_kv(layer, None if self._k_out is None else self._k_out[:n], v[:n])
 
     def _ws(self):
         """Workspace of the dense calls, made by the first of them (a captured
