@@ -723,7 +723,8 @@ int32_t locks_qkv_write(const uint16_t* q, int64_t q_stride_tok, int64_t q_strid
  *   in masked places of the cache (unwritten pages, tokens out of the window or
  *   after the query), NaN and infinities included, does not matter.
  *   scale > 0.  fp32 scores, softmax and sums; the weights are rounded to bf16
- *   for the product with V.
+ *   for the product with V.  They are normalised at the end and at most 2^8 before:
+ *   max |V| x visible keys x 2^8 has to stay within fp32.
  *   max_seq_len  host-side upper bound of seq_lens (0: the table's width); only
  *                sizes the launch
  *   workspace    16-byte aligned device memory, workspace_bytes >= what the call
@@ -770,7 +771,8 @@ int32_t locks_window_prefill(const uint16_t* q, int64_t q_stride_tok, int64_t q_
  * table row of a member that is as long as the prefix (of its longest one where
  * none is); the rows of shorter members and of padding may hold anything past
  * their own pages.  A member shorter than the prefix sees only its own length.  A
- * request in no group is attended like any other.
+ * request in no group is attended like any other; n_groups >= 1, a group may hold
+ * no request.
  *   max_prefix_pages  host-side upper bound of prefix_pages (0: none); only sizes
  *                     the launch */
 int32_t locks_prefix_decode(const uint16_t* q, int64_t q_stride_req, int64_t q_stride_head,

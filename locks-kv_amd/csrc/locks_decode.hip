@@ -278,7 +278,7 @@ struct TierSrc {
 // RANGE (with DENSE's contiguous steps): the tokens of RangeSrc, split by
 // 16-token steps instead of pages.  P stays bf16 like V, so that V's whole range
 // holds, and V rows that the range leaves out count as zero, whatever they hold.  32
-// ragged requests of a window of 8192: 89 us, 6.0 TB/s; one of 4096: 8.3 us, a chain
+// ragged requests of a window of 8192: 89-90 us, 6.0 TB/s; one of 4096: 8.3 us, a chain
 // of length, ids, two steps a wave and the join.
 template <bool FUSED, bool DENSE = false, int NST = 2, int KVPOL = 0, int D = 128, bool TIER = false,
           bool RANGE = false>
@@ -1135,7 +1135,9 @@ int launch_decode_range(const uint16_t* q, long q_sr, long q_sh, const uint16_t*
                         const Partials& p, const RangeSrc& range, int nsplit, int min_steps, int n_req, int n_kv, int G,
                         int head_dim, int page, float scale, hipStream_t stream) {
     const int pg_sh = page == 16 ? 0 : page == 32 ? 1 : 2;
-#define LAUNCH_D(DV)                                                                                                  hipLaunchKernelGGL((decode_split_kernel<false, true, DENSE_NST, CPOL_NT, DV, false, true>),                                          dim3(nsplit, n_kv, n_req), dim3(DC_BLK), 0, stream, q, q_sr, q_sh, k, ks[0], ks[1], ks[2], \
+#define LAUNCH_D(DV)                                                                                             \
+    hipLaunchKernelGGL((decode_split_kernel<false, true, DENSE_NST, CPOL_NT, DV, false, true>),                   \
+                       dim3(nsplit, n_kv, n_req), dim3(DC_BLK), 0, stream, q, q_sr, q_sh, k, ks[0], ks[1], ks[2], \
                        v, vs[0], vs[1], vs[2], num_blocks, bt, bt_sr, bt_cols, nullptr, 0L, 0L, 1, nullptr, 0L,   \
                        seq_lens, p.m, p.l, p.acc, G, p.splits, min_steps, scale, pg_sh, nullptr, nullptr, 0L, 0L, \
                        0, range)

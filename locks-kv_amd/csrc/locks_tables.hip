@@ -15,8 +15,9 @@
 // bytes that stay in the cache) instead of waiting for another kernel, then
 // takes its share of the page ids and of the tokens.  lens and head change in
 // place, so the last workgroup to have read them writes them (an arrival count,
-// left at zero).  Bound by latency: two dependent loads (row, then its length)
-// before the sums, and the copy of the page ids after them.  32 requests of up to 2048
+// left at zero).  Bound by latency: the rows are read three times, twice for the
+// claims with a barrier behind each, then the lengths, three prefix sums of two
+// barriers each, the arrival, and the copy of the page ids.  32 requests of up to 2048
 // pages 6.2 us, 256 of up to 4096 with 16K tokens 11.4, the roll-back 4.4-4.7.
 #include "locks_common.h"
 #include "locks_hip.h"

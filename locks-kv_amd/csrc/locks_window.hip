@@ -20,11 +20,14 @@
 // K and V arrive by direct loads to LDS, one tile ahead (two at d 64 and 256).
 // 16-byte chunks of a row are permuted by the row on the way in (an exclusive or),
 // which keeps the reads of both operands free of bank conflicts.
-// 8192 tokens, 32 / 8 heads, d 128, causal: 556 us, 989 TFLOP/s, the matrix cores
-// 42-45 % busy; copies for timing: without the softmax 496, without K and V reads
-// from LDS too 440, without staging too 353.  64 keys a tile and 4 waves: 32 keys
-// with four tiles in LDS took 580, 8 waves on 256 rows 548 there but 163 for 139 at
-// d 64 and 96 for 77 on a prefix.
+// 8192 tokens, 32 / 8 heads, d 128, causal: 548 to 616 us over four cards, 1003 to 892
+// TFLOP/s, the matrix cores 42-45 % busy: a wave does scores, softmax and V's
+// products in turn, and only its SIMD's other wave fills the gaps (at d 64 the time
+// is near the sum of products and softmax).  On a card of 556, copies for timing:
+// without the softmax 496, without K and V reads from LDS too 440, without staging too
+// 353.  64 keys a tile and 4 waves (577 on a third card): 32 keys with four tiles in
+// LDS took 580 there, 8 waves on 256 rows 548 but 163 for 139 at d 64 and 96 for 77 on
+// a prefix.
 //
 // Decode (one token): the split kernel of locks_decode.hip over a token range, or
 // (with a shared prefix) the tiles above, of which a request fills one column block.
@@ -329,8 +332,10 @@ __global__ __launch_bounds__(AT_BLK, D == 256 ? 1 : 2) void attn_tile_kernel(con
             for (int kb2 = 0; kb2 < NB2; ++kb2)
                 s[kb2] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[kb2][st], qf[st], s[kb2], 0, 0, 0);
     };
-    // The running maximum and sum, O^T rescaled where a maximum grew; P in bf16
-    // (half a step 2^-8 of each weight; l keeps the unrounded ones), PV's operand
+    // The running maximum and sum, O^T rescaled where a maximum grew; P in bf16, PV's
+    // operand: the product takes two operands of one type, and V in fp16 would lose
+    // its range.  Half a step, 2^-8 of each weight; l keeps the unrounded ones.
+    // (Outputs against 64 bits: 2.2e-3, with weights in fp32 1.6e-3.)
     auto weights = [&](const v16f* s, v8bf* pf) __attribute__((always_inline)) {
         float mx = s[0][0];
 #pragma unroll
@@ -620,7 +625,9 @@ static int clampi(long x, int lo, int hi) { return (int)(x < lo ? lo : x > hi ? 
 // A single-token call: about 512 workgroups (two per CU), each of at least 8
 // 16-token steps (two per wave).  With `even`, a row's splits hold at most 64 steps:
 // lengths differ, and the longest split is the call's time (32 ragged requests of a
-// window of 8192: 119 us at 2 splits, 96.5 at 9, 103 at 17), up to 4096 workgroups.
+// window of 8192, all on one card when the rule was set: 119 us at 2 splits, 96.5 at
+// 9, 103 at 17; 93-94 now), up to 4096 workgroups.  64 splits at most: one row of 1M
+// tokens at two kv heads has 128 workgroups on 256 CUs.
 static int decode_splits(int n_req, int n_kv, long max_keys, bool even) {
     const long rows = (long)n_req * n_kv, steps = (max_keys + 15) / 16;
     const long fill = (512 + rows - 1) / rows, cap = (4096 + rows - 1) / rows;

@@ -149,7 +149,8 @@ def prefix_decode(q, kv_cache, block_table, seq_lens, group_start, prefix_pages,
     the row of a member that is as long (of the longest where none is).  Both are
     int32 on the GPU, so that a captured call follows them.  Requests outside all
     groups, members shorter than the prefix and padding (length 0) are attended
-    like any other; their rows need hold no more pages than their lengths."""
+    like any other; their rows need hold no more pages than their lengths.
+    ``n_groups`` is at least 1; a group may hold no request."""
     head, tail, geo, index = _args("prefix_decode", q, kv_cache, block_table, seq_lens, out, ws, lse, n_req, n_req)
     _i32("prefix_decode: group_start", group_start, n_groups + 1, index)
     _i32("prefix_decode: prefix_pages", prefix_pages, n_groups, index)
