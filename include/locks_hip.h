@@ -41,7 +41,7 @@
 
 #include <stdint.h>
 
-#define LOCKS_ABI_VERSION 11
+#define LOCKS_ABI_VERSION 12
 #define LOCKS_TABLES_MAX_REQS 2048
 
 #ifdef __cplusplus
@@ -788,6 +788,85 @@ int32_t locks_prefix_decode(const uint16_t* q, int64_t q_stride_req, int64_t q_s
                             int32_t max_prefix_pages, int32_t max_seq_len, float scale,
                             void* stream);
 
+/*
+ * locks_qkv_write for positions of several axes (time, height, width): positions
+ * (n_axes, n_tokens) i32, pos_stride_axis elements apart, 1 <= n_axes <= 4; pair j
+ * of a head's first rot entries turns by the angle cos_sin[position of axis a(j)][j].
+ * a(j) is bits 2 (j & 31) and 2 (j & 31) + 1 of the word axes<j >> 5>, and below
+ * n_axes.  A token with a position of any axis outside [0, max_pos) is treated as one
+ * whose position is.
+ */
+int32_t locks_qkv_write_axes(const uint16_t* q, int64_t q_stride_tok, int64_t q_stride_head,
+                             const uint16_t* k, int64_t k_stride_tok, int64_t k_stride_head,
+                             const uint16_t* v, int64_t v_stride_tok, int64_t v_stride_head,
+                             const int32_t* positions, int64_t pos_stride_axis, int32_t n_axes,
+                             int64_t axes0, int64_t axes1, int64_t axes2, int64_t axes3,
+                             const int64_t* slot_mapping, uint16_t* k_cache, int64_t kc_stride_block,
+                             int64_t kc_stride_tok, int64_t kc_stride_head, uint16_t* v_cache,
+                             int64_t vc_stride_block, int64_t vc_stride_tok, int64_t vc_stride_head,
+                             int32_t num_blocks, const float* cos_sin, int32_t max_pos, int32_t rot,
+                             int32_t interleaved, const void* q_weight, const void* k_weight,
+                             int32_t weights_f32, float eps, uint16_t* q_out, int64_t qo_stride_tok,
+                             int64_t qo_stride_head, uint16_t* k_out, int64_t ko_stride_tok,
+                             int64_t ko_stride_head, int32_t n_tokens, int32_t n_heads, int32_t n_kv,
+                             int32_t head_dim, int32_t page, void* stream);
+
+/*
+ * The paged cache in 4 bits.  32 consecutive entries of one head of one token share
+ * a scale 2^e, e the smallest whole number of [-125, 125] with max |x| <= 7 * 2^e,
+ * and each is the nearest of +-{0, 0.5, 1, 1.5, 2, 3, 4, 6} 2^e, ties to the even one
+ * of the eight (larger ones, past 7 * 2^125: 6 * 2^125).  32 entries with an infinite
+ * or NaN one among them read as NaN.
+ *   cache   (num_blocks, n_kv) records of page / 16 tiles of 17 * head_dim bytes, one
+ *           after the other; strides of block and kv head in bytes, multiples of 16,
+ *           the base 16-byte aligned.  A tile's layout is locks_kv4.h's.
+ *
+ * locks_kv4_write   locks_qkv_write (n_axes 0) or locks_qkv_write_axes into such a
+ *           cache; keys are rounded from their norm and rotation in 64 bits, k_out
+ *           holds them in bf16.
+ * locks_kv4_read    rows slots[t] = block * page + offset as bf16, exactly (k_out, v_out
+ *           (n_tokens, n_kv, d)); a slot outside the cache leaves its rows as they were.
+ * locks_kv4_decode, locks_kv4_prefill   locks_window_decode and locks_window_prefill
+ *           over the values of such a cache, with the same workspace.
+ */
+int32_t locks_kv4_write(const uint16_t* q, int64_t q_stride_tok, int64_t q_stride_head,
+                        const uint16_t* k, int64_t k_stride_tok, int64_t k_stride_head,
+                        const uint16_t* v, int64_t v_stride_tok, int64_t v_stride_head,
+                        const int32_t* positions, int64_t pos_stride_axis, int32_t n_axes,
+                        int64_t axes0, int64_t axes1, int64_t axes2, int64_t axes3,
+                        const int64_t* slot_mapping, uint8_t* cache, int64_t c_stride_block,
+                        int64_t c_stride_head, int32_t num_blocks, const float* cos_sin,
+                        int32_t max_pos, int32_t rot, int32_t interleaved, const void* q_weight,
+                        const void* k_weight, int32_t weights_f32, float eps, uint16_t* q_out,
+                        int64_t qo_stride_tok, int64_t qo_stride_head, uint16_t* k_out,
+                        int64_t ko_stride_tok, int64_t ko_stride_head, int32_t n_tokens,
+                        int32_t n_heads, int32_t n_kv, int32_t head_dim, int32_t page, void* stream);
+
+int32_t locks_kv4_read(const uint8_t* cache, int64_t c_stride_block, int64_t c_stride_head,
+                       int32_t num_blocks, const int64_t* slots, uint16_t* k_out,
+                       int64_t k_stride_tok, int64_t k_stride_head, uint16_t* v_out,
+                       int64_t v_stride_tok, int64_t v_stride_head, int32_t n_tokens, int32_t n_kv,
+                       int32_t head_dim, int32_t page, void* stream);
+
+int32_t locks_kv4_decode(const uint16_t* q, int64_t q_stride_req, int64_t q_stride_head,
+                         const uint8_t* cache, int64_t c_stride_block, int64_t c_stride_head,
+                         int32_t num_blocks, const int32_t* block_table, int64_t bt_stride,
+                         int32_t bt_cols, const int32_t* seq_lens, int32_t window, int32_t sinks,
+                         uint16_t* out, int64_t out_stride_req, int64_t out_stride_head, float* lse,
+                         int64_t lse_stride_req, void* workspace, int64_t workspace_bytes,
+                         int32_t n_req, int32_t n_kv, int32_t G, int32_t head_dim, int32_t page,
+                         int32_t max_seq_len, float scale, void* stream);
+
+int32_t locks_kv4_prefill(const uint16_t* q, int64_t q_stride_tok, int64_t q_stride_head,
+                          const uint8_t* cache, int64_t c_stride_block, int64_t c_stride_head,
+                          int32_t num_blocks, const int32_t* block_table, int64_t bt_stride,
+                          int32_t bt_cols, const int32_t* seq_lens, const int32_t* query_start_loc,
+                          int32_t window, int32_t sinks, uint16_t* out, int64_t out_stride_tok,
+                          int64_t out_stride_head, float* lse, int64_t lse_stride_tok,
+                          void* workspace, int64_t workspace_bytes, int32_t n_tokens, int32_t n_req,
+                          int32_t n_kv, int32_t G, int32_t head_dim, int32_t page,
+                          int32_t max_seq_len, float scale, void* stream);
+
 /* The entries of a serving step with their arguments as n 8-byte words in order
  * (integers and pointers as they are, floats as doubles; an integer past its
  * argument's 32 bits is refused): for bindings where every argument of a foreign
@@ -798,6 +877,11 @@ int32_t locks_prefix_decode(const uint16_t* q, int64_t q_stride_req, int64_t q_s
 #define LOCKS_CALL_WINDOW_DECODE 3
 #define LOCKS_CALL_WINDOW_PREFILL 4
 #define LOCKS_CALL_PREFIX_DECODE 5
+#define LOCKS_CALL_QKV_WRITE_AXES 6
+#define LOCKS_CALL_KV4_WRITE 7
+#define LOCKS_CALL_KV4_READ 8
+#define LOCKS_CALL_KV4_DECODE 9
+#define LOCKS_CALL_KV4_PREFILL 10
 int32_t locks_call(int32_t entry, const uint64_t* words, int32_t n);
 
 #ifdef __cplusplus

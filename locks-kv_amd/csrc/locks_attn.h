@@ -43,4 +43,32 @@ int launch_decode_range(const uint16_t* q, long q_sr, long q_sh, const uint16_t*
                         const Partials& p, const RangeSrc& range, int nsplit, int min_steps, int n_req, int n_kv, int G,
                         int head_dim, int page, float scale, hipStream_t stream);
 
+constexpr int AT_MAX_SPLITS = 128;          // of one row, all kinds together
+
+// Joins the partials of every row (locks_window.hip); with `starts` only of the rows
+// of starts[0] .. starts[n_seq].
+int launch_merge(const Partials& p, uint16_t* out, long o_st, long o_sh, float* lse, long lse_st, int n_tok, int n_kv,
+                 int G, int head_dim, const int* starts, int n_seq, hipStream_t st);
+
+// Bytes of a call's partials, and where they stand in its workspace.
+inline int64_t part_bytes(int64_t rows, int splits, int D) { return rows * splits * (D + 2) * 4; }
+inline Partials part_layout(void* ws, int64_t rows, int splits, int D) {
+    float* acc = static_cast<float*>(ws);   // first: 16-byte aligned
+    return Partials{acc + rows * splits * D, acc + rows * splits * (D + 1), acc, splits};
+}
+
+// What every attention entry asks of its arguments, and of its workspace.
+int32_t check_attn(const char* what, const uint16_t* q, int64_t q_st, int64_t q_sh, const uint16_t* k,
+                   const int64_t* ks, const uint16_t* v, const int64_t* vs, int32_t num_blocks, const int32_t* bt,
+                   int64_t bt_stride, int32_t bt_cols, const int32_t* seq_lens, int32_t window, int32_t sinks,
+                   const uint16_t* out, int64_t o_st, int64_t o_sh, int32_t n_req, int32_t n_kv, int32_t G,
+                   int32_t head_dim, int32_t page, int32_t max_keys, float scale);
+int32_t check_ws(const char* what, const void* ws, int64_t have, int64_t need);
+// And of a cache in 4 bits (locks_kv4.hip).
+int32_t check_kv4(const char* what, const void* cache, int64_t sb, int64_t sh, int32_t num_blocks, int32_t n_kv,
+                  int32_t head_dim, int32_t page);
+
+// Workgroups of a row of a single-token call on a cache in 4 bits (locks_kv4.hip).
+int kv4_decode_splits(int n_req, int n_kv, long max_keys);
+
 }  // namespace locks

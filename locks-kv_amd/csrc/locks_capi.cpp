@@ -93,6 +93,11 @@ extern "C" int32_t locks_call(int32_t entry, const uint64_t* words, int32_t n) {
         case LOCKS_CALL_WINDOW_DECODE: return call_with(locks_window_decode, words, n);
         case LOCKS_CALL_WINDOW_PREFILL: return call_with(locks_window_prefill, words, n);
         case LOCKS_CALL_PREFIX_DECODE: return call_with(locks_prefix_decode, words, n);
+        case LOCKS_CALL_QKV_WRITE_AXES: return call_with(locks_qkv_write_axes, words, n);
+        case LOCKS_CALL_KV4_WRITE: return call_with(locks_kv4_write, words, n);
+        case LOCKS_CALL_KV4_READ: return call_with(locks_kv4_read, words, n);
+        case LOCKS_CALL_KV4_DECODE: return call_with(locks_kv4_decode, words, n);
+        case LOCKS_CALL_KV4_PREFILL: return call_with(locks_kv4_prefill, words, n);
         default: locks::set_error("locks_call: no entry %d", entry); return -1;
     }
 }

@@ -15,8 +15,10 @@
 // comes over with four permutes and is normed again here).  Bound by memory: every
 // row is read and written once.  8192 tokens of 32 + 16 heads of 128: 41 us, 5.0 TB/s,
 // a copy's rate; one token 3.8 us.
+#include "locks_attn.h"
 #include "locks_common.h"
 #include "locks_hip.h"
+#include "locks_kv4.h"
 
 namespace locks {
 
@@ -37,7 +39,12 @@ struct QkvArgs {
     long slots;                             // num_blocks * page
     int max_pos, rot, n_tok, H, n_kv, pg_sh, groups;
     float eps;
+    // AXES: positions of n_axes axes, pos_ax apart, and each pair's axis in two bits
+    int n_axes; long pos_ax;
+    uint64_t axes[4];
+    uint8_t* c4; long c_sb, c_sh;           // KV4: the cache, in place of kc and vc
 };
+constexpr int QK_AXES = 4;
 
 __device__ __forceinline__ void unpack8(const uint4& w, float* x) {
     x[0] = bf16lo(w.x); x[1] = bf16hi(w.x); x[2] = bf16lo(w.y); x[3] = bf16hi(w.y);
@@ -84,7 +91,58 @@ __device__ __forceinline__ float head_sum(float s) {
     return s;
 }
 
-template <int D, int IT, bool INTER, bool WF32>
+// ---- a cache in 4 bits ----------------------------------------------------------
+// Codes are steps of a whole exponent apart, so that a value next to a border decides
+// a step: the keys' norm and rotation are done in 64 bits (their few heads' arithmetic
+// is a small part of a call that memory bounds), and a code is the same wherever the
+// exact value is.
+template <int D>
+__device__ __forceinline__ double head_sum(double s) {
+#pragma unroll
+    for (int x = D / 16; x >= 1; x >>= 1) s += __shfl_xor(s, x);
+    return s;
+}
+// The largest exponent word of the four lanes that share a scale.
+__device__ __forceinline__ uint32_t block_max(uint32_t x) {
+    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0xB1, 0xF, 0xF, false));    // lane ^ 1
+    return max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x4E, 0xF, 0xF, false));  // lane ^ 2
+}
+// e of a block's largest magnitude, from the leading 32 bits of its double (rounded
+// up to the next where lower bits are set: 7 * 2^e is 0x..1C00000000000).
+__device__ __forceinline__ int block_exp(uint32_t hi) {
+    const int e = (int)(hi >> 20) - 1023 - 2 + ((hi & 0xFFFFFu) > 0xC0000u ? 1 : 0);
+    return min(max(e, -125), 125);
+}
+__device__ __forceinline__ uint32_t top_bits(double x) {
+    const uint64_t u = (uint64_t)__double_as_longlong(x) & 0x7FFFFFFFFFFFFFFFull;
+    return (uint32_t)(u >> 32) + ((uint32_t)u ? 1u : 0u);
+}
+// To fp32 with the last bit set where the value is not exact: whatever rounds to fewer
+// bits from there, rounds as from 64.
+__device__ __forceinline__ float to_odd(double y) {
+    const float f = (float)y;
+    const double d = y - (double)f;
+    uint32_t u = __float_as_uint(f);
+    if (d != 0.0 && !(u & 1)) u += (d > 0.0) != (bool)(u >> 31) ? 1u : -1u;
+    return __uint_as_float(u);
+}
+// Eight entries over 2^e as codes, and the scale's byte.
+__device__ __forceinline__ uint32_t to_codes(const double* x, uint32_t& byte) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) top = max(top, top_bits(x[e]));
+    top = block_max(top);
+    const int ex = block_exp(top);
+    byte = top >= 0x7FF00000u ? 255u : (uint32_t)(ex + 127);
+    const double inv = __longlong_as_double((long long)(1023 - ex) << 52);
+    uint32_t w = 0;
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, to_odd(x[0] * inv), to_odd(x[1] * inv), 1.f, 0);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, to_odd(x[2] * inv), to_odd(x[3] * inv), 1.f, 1);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, to_odd(x[4] * inv), to_odd(x[5] * inv), 1.f, 2);
+    return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, to_odd(x[6] * inv), to_odd(x[7] * inv), 1.f, 3);
+}
+
+template <int D, int IT, bool INTER, bool WF32, bool AXES, bool KV4>
 __global__ __launch_bounds__(QK_BLK) void qkv_write_kernel(const QkvArgs a)
 {
     constexpr int LPH = D / 8, HPW = kWave / LPH;       // lanes per head, heads per wave
@@ -112,25 +170,41 @@ __global__ __launch_bounds__(QK_BLK) void qkv_write_kernel(const QkvArgs a)
         // past the caches too: 42.5 alone, but 134 with the attention)
         raw[i] = __builtin_bit_cast(uint4, __builtin_nontemporal_load(reinterpret_cast<const v4i*>(p + e0)));
     }
-    const int pos = a.pos[t];
+    int pos[AXES ? QK_AXES : 1];
+    bool placed = true;
+#pragma unroll
+    for (int x = 0; x < (AXES ? QK_AXES : 1); ++x) {
+        pos[x] = a.pos[t + (AXES ? min(x, a.n_axes - 1) * a.pos_ax : 0)];
+        placed = placed && pos[x] >= 0 && pos[x] < a.max_pos;
+    }
     const long slot = a.slot[t];
-    const bool placed = pos >= 0 && pos < a.max_pos;
     const int half = a.rot >> 1;
     const bool turned = e0 < a.rot;
     // angles of this lane's entries (8 pairs, or 4 adjacent ones); the partner lane of a half-split pair
     float c[8], s[8];
     const bool low = e0 < half;
     const int pl = (lane & ~(LPH - 1)) + (low ? l + half / 8 : l - half / 8);
-    const float* row = a.cs + (long)(placed ? pos : 0) * a.rot;
     if (turned) {
         const int j = INTER ? e0 >> 1 : low ? e0 : e0 - half;
         constexpr int N = INTER ? 4 : 8;
+        // AXES: the same entries of every axis' row, and each pair takes its axis'
+        const uint32_t ax = AXES ? (uint32_t)(a.axes[j >> 5] >> (2 * (j & 31))) : 0;
 #pragma unroll
-        for (int e = 0; e < N; e += 4) {
-            const float4 x = *reinterpret_cast<const float4*>(row + j + e);
-            const float4 y = *reinterpret_cast<const float4*>(row + half + j + e);
-            c[e] = x.x; c[e + 1] = x.y; c[e + 2] = x.z; c[e + 3] = x.w;
-            s[e] = y.x; s[e + 1] = y.y; s[e + 2] = y.z; s[e + 3] = y.w;
+        for (int x = 0; x < (AXES ? QK_AXES : 1); ++x) {
+            if (AXES && x >= a.n_axes) break;
+            const float* row = a.cs + (long)(placed ? pos[x] : 0) * a.rot;
+#pragma unroll
+            for (int e = 0; e < N; e += 4) {
+                const float4 u4 = *reinterpret_cast<const float4*>(row + j + e);
+                const float4 w4 = *reinterpret_cast<const float4*>(row + half + j + e);
+                const float cu[4] = {u4.x, u4.y, u4.z, u4.w}, sw[4] = {w4.x, w4.y, w4.z, w4.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const bool here = !AXES || x == 0 || ((ax >> (2 * (e + i))) & 3) == (uint32_t)x;
+                    c[e + i] = here ? cu[i] : c[e + i];
+                    s[e + i] = here ? sw[i] : s[e + i];
+                }
+            }
         }
     }
     // weights of this lane's entries and of its partner's, for q and for k
@@ -183,15 +257,75 @@ __global__ __launch_bounds__(QK_BLK) void qkv_write_kernel(const QkvArgs a)
                 for (int e = 0; e < 8; ++e) x[e] = low ? x[e] * c[e] - y[e] * s[e] : x[e] * c[e] + y[e] * s[e];
             }
         }
+        if constexpr (KV4) {
+            // (waves that hold no head of K or V are through with it here)
+            if (cached && u[i] >= a.H && u[i] < NU) {
+                const int h = (is_k ? u[i] - a.H : u[i] - a.H - a.n_kv);
+                uint8_t* tile = a.c4 + blk * a.c_sb + (long)h * a.c_sh + (off >> 4) * Kv4<D>::TILE;
+                const int key = off & 15;
+                float r8[8], rp[8];
+                unpack8(raw[i], r8);
+                unpack8(pr, rp);
+                double z[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) z[e] = r8[e];
+                if (is_k) {
+                    double sum = 0.0;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) sum += z[e] * z[e];
+                    sum = head_sum<D>(sum);
+                    double f = 1.0, p[8];
+                    float g[8], gp[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) { p[e] = rp[e]; g[e] = gp[e] = 1.f; }
+                    if (normed) {
+                        f = 1.0 / sqrt(sum * (1.0 / D) + (double)a.eps);
+                        wk.get(g);
+                        pk.get(gp);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) { z[e] *= f * (double)g[e]; p[e] *= f * (double)gp[e]; }
+                    if (turned) {
+                        if constexpr (INTER) {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const double zx = z[2 * e], zy = z[2 * e + 1];
+                                z[2 * e] = zx * (double)c[e] - zy * (double)s[e];
+                                z[2 * e + 1] = zy * (double)c[e] + zx * (double)s[e];
+                            }
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 8; ++e)
+                                z[e] = low ? z[e] * (double)c[e] - p[e] * (double)s[e] : z[e] * (double)c[e] + p[e] * (double)s[e];
+                        }
+                    }
+                }
+                uint32_t byte;
+                const uint32_t w = to_codes(z, byte);
+                if (is_k) {
+                    *reinterpret_cast<uint32_t*>(tile + Kv4<D>::k_code(key, l)) = w;
+                    if ((l & 3) == 0) tile[Kv4<D>::k_scale(key, l >> 2)] = (uint8_t)byte;
+                } else {
+                    uint8_t* p4 = tile + Kv4<D>::v_code(key, l);
+                    if constexpr (D == 64) {
+                        *reinterpret_cast<uint16_t*>(p4) = (uint16_t)w;
+                        *reinterpret_cast<uint16_t*>(p4 + 8) = (uint16_t)(w >> 16);
+                    } else {
+                        *reinterpret_cast<uint32_t*>(p4) = w;
+                    }
+                    if ((l & 3) == 0) tile[Kv4<D>::v_scale(key, l >> 2)] = (uint8_t)byte;
+                }
+            }
+        }
         uint4 out = pack8(x);
         if (!placed) out = make_uint4(0x7FC07FC0u, 0x7FC07FC0u, 0x7FC07FC0u, 0x7FC07FC0u);
         if (u[i] < a.H) {
             *reinterpret_cast<uint4*>(a.qo + (long)t * a.qo_st + (long)u[i] * a.qo_sh + e0) = out;
         } else if (u[i] < a.H + a.n_kv) {
             const int h = u[i] - a.H;
-            if (cached) *reinterpret_cast<uint4*>(a.kc + blk * a.kc_sb + (long)off * a.kc_st + (long)h * a.kc_sh + e0) = out;
+            if (cached && !KV4) *reinterpret_cast<uint4*>(a.kc + blk * a.kc_sb + (long)off * a.kc_st + (long)h * a.kc_sh + e0) = out;
             if (a.ko) *reinterpret_cast<uint4*>(a.ko + (long)t * a.ko_st + (long)h * a.ko_sh + e0) = out;
-        } else if (u[i] < NU && cached) {
+        } else if (u[i] < NU && cached && !KV4) {
             const int h = u[i] - a.H - a.n_kv;
             *reinterpret_cast<uint4*>(a.vc + blk * a.vc_sb + (long)off * a.vc_st + (long)h * a.vc_sh + e0) = raw[i];
         }
@@ -201,6 +335,124 @@ __global__ __launch_bounds__(QK_BLK) void qkv_write_kernel(const QkvArgs a)
 }  // namespace locks
 
 using namespace locks;
+
+namespace {
+
+// The strides and pointers of a call, whatever its cache.
+int32_t check_qkv(const char* what, const QkvArgs& a, int head_dim, int page, int num_blocks)
+{
+    LOCKS_REQUIRE(head_dim == 64 || head_dim == 128 || head_dim == 256, "%s: head_dim %d outside {64, 128, 256}", what, head_dim);
+    LOCKS_REQUIRE(page == 16 || page == 32 || page == 64, "%s: page %d outside {16, 32, 64}", what, page);
+    LOCKS_REQUIRE(a.rot >= 0 && a.rot <= head_dim && a.rot % 16 == 0,
+                  "%s: rot %d is not a multiple of 16 in [0, head_dim %d]", what, a.rot, head_dim);
+    LOCKS_REQUIRE(a.n_tok >= 0 && a.H >= 1 && a.n_kv >= 1 && num_blocks >= 1 && a.max_pos >= 1, "%s: empty geometry", what);
+    LOCKS_REQUIRE(a.H <= 4096 && a.n_kv <= 4096, "%s: more than 4096 heads", what);
+    LOCKS_REQUIRE(a.eps >= 0.f, "%s: eps must not be negative", what);
+    LOCKS_REQUIRE(a.q && a.k && a.v && a.pos && a.slot && (a.c4 || (a.kc && a.vc)) && a.qo && (a.cs || a.rot == 0),
+                  "%s: null pointer argument", what);
+    for (int64_t x : {a.q_st, a.q_sh, a.k_st, a.k_sh, a.v_st, a.v_sh, a.kc_sb, a.kc_st, a.kc_sh, a.vc_sb, a.vc_st, a.vc_sh,
+                      a.qo_st, a.qo_sh, a.ko_st, a.ko_sh})
+        LOCKS_REQUIRE(x % 8 == 0, "%s: strides must be multiples of 8 elements (16-byte accesses)", what);
+    for (const void* x : {(const void*)a.q, (const void*)a.k, (const void*)a.v, (const void*)a.kc, (const void*)a.vc,
+                          (const void*)a.qo, (const void*)a.ko, (const void*)a.cs, a.qw, a.kw})
+        LOCKS_REQUIRE((uintptr_t)x % 16 == 0, "%s: pointers must be 16-byte aligned", what);
+    return 0;
+}
+int32_t check_axes(const char* what, QkvArgs& a, int32_t n_axes, int64_t pos_stride, const int64_t (&words)[4])
+{
+    LOCKS_REQUIRE(n_axes >= 0 && n_axes <= QK_AXES, "%s: n_axes %d outside [0, %d]", what, n_axes, QK_AXES);
+    if (n_axes == 0) return 0;
+    uint64_t axes[4];
+    for (int i = 0; i < 4; ++i) axes[i] = (uint64_t)words[i];
+    for (int j = 0; j < a.rot / 2; ++j)
+        LOCKS_REQUIRE((int)(axes[j >> 5] >> (2 * (j & 31)) & 3) < n_axes, "%s: pair %d turns by an axis past the %d", what, j, n_axes);
+    a.n_axes = n_axes;
+    a.pos_ax = pos_stride;
+    for (int i = 0; i < 4; ++i) a.axes[i] = axes[i];
+    return 0;
+}
+
+template <bool KV4>
+int32_t launch_qkv(QkvArgs a, int head_dim, int interleaved, int weights_f32, hipStream_t st)
+{
+    if (a.n_tok == 0) return 0;
+    a.groups = cdiv(a.H + 2 * a.n_kv, 512 / head_dim);
+    // groups per wave: the angles and weights of a token are loaded once for them,
+    // and their rows are in flight together (8192 tokens of 48 heads: 2 groups 50.5
+    // us, 3 and 4 45)
+    constexpr int IT = 3;
+    const long waves = (long)a.n_tok * cdiv(a.groups, IT);
+    const dim3 grid((unsigned)((waves + QK_WAVES - 1) / QK_WAVES));
+#define LAUNCH_A(DV, INTER, WF32)                                                                                          \
+    if (a.n_axes) hipLaunchKernelGGL((qkv_write_kernel<DV, IT, INTER, WF32, true, KV4>), grid, dim3(QK_BLK), 0, st, a);    \
+    else hipLaunchKernelGGL((qkv_write_kernel<DV, IT, INTER, WF32, false, KV4>), grid, dim3(QK_BLK), 0, st, a)
+#define LAUNCH_W(DV, INTER)                               \
+    if (weights_f32) { LAUNCH_A(DV, INTER, true); }       \
+    else { LAUNCH_A(DV, INTER, false); }
+#define LAUNCH(DV)                              \
+    if (interleaved) { LAUNCH_W(DV, true); }    \
+    else { LAUNCH_W(DV, false); }
+    if (head_dim == 64) { LAUNCH(64); }
+    else if (head_dim == 128) { LAUNCH(128); }
+    else { LAUNCH(256); }
+#undef LAUNCH
+#undef LAUNCH_W
+#undef LAUNCH_A
+    return check_launch("qkv_write_kernel");
+}
+
+int page_shift(int page) { return page == 16 ? 4 : page == 32 ? 5 : 6; }
+
+}  // namespace
+
+extern "C" int32_t locks_qkv_write_axes(
+    const uint16_t* q, int64_t q_stride_tok, int64_t q_stride_head, const uint16_t* k, int64_t k_stride_tok,
+    int64_t k_stride_head, const uint16_t* v, int64_t v_stride_tok, int64_t v_stride_head, const int32_t* positions,
+    int64_t pos_stride_axis, int32_t n_axes, int64_t axes0, int64_t axes1, int64_t axes2, int64_t axes3,
+    const int64_t* slot_mapping, uint16_t* k_cache, int64_t kc_stride_block, int64_t kc_stride_tok,
+    int64_t kc_stride_head, uint16_t* v_cache, int64_t vc_stride_block, int64_t vc_stride_tok, int64_t vc_stride_head,
+    int32_t num_blocks, const float* cos_sin, int32_t max_pos, int32_t rot, int32_t interleaved, const void* q_weight,
+    const void* k_weight, int32_t weights_f32, float eps, uint16_t* q_out, int64_t qo_stride_tok,
+    int64_t qo_stride_head, uint16_t* k_out, int64_t ko_stride_tok, int64_t ko_stride_head, int32_t n_tokens,
+    int32_t n_heads, int32_t n_kv, int32_t head_dim, int32_t page, void* stream)
+{
+    const char* what = "locks_qkv_write_axes";
+    QkvArgs a{q, q_stride_tok, q_stride_head, k, k_stride_tok, k_stride_head, v, v_stride_tok, v_stride_head,
+              positions, slot_mapping, k_cache, kc_stride_block, kc_stride_tok, kc_stride_head, v_cache,
+              vc_stride_block, vc_stride_tok, vc_stride_head, cos_sin, q_weight, k_weight, q_out, qo_stride_tok,
+              qo_stride_head, k_out, ko_stride_tok, ko_stride_head, (long)num_blocks * page, max_pos, rot,
+              n_tokens, n_heads, n_kv, page_shift(page), 0, eps, 0, 0, {}, nullptr, 0, 0};
+    int rc = check_qkv(what, a, head_dim, page, num_blocks);
+    if (rc) return rc;
+    LOCKS_REQUIRE(n_axes >= 1, "%s: n_axes %d outside [1, %d]", what, n_axes, QK_AXES);
+    rc = check_axes(what, a, n_axes, pos_stride_axis, {axes0, axes1, axes2, axes3});
+    if (rc) return rc;
+    return launch_qkv<false>(a, head_dim, interleaved, weights_f32, (hipStream_t)stream);
+}
+
+extern "C" int32_t locks_kv4_write(
+    const uint16_t* q, int64_t q_stride_tok, int64_t q_stride_head, const uint16_t* k, int64_t k_stride_tok,
+    int64_t k_stride_head, const uint16_t* v, int64_t v_stride_tok, int64_t v_stride_head, const int32_t* positions,
+    int64_t pos_stride_axis, int32_t n_axes, int64_t axes0, int64_t axes1, int64_t axes2, int64_t axes3,
+    const int64_t* slot_mapping, uint8_t* cache, int64_t c_stride_block, int64_t c_stride_head, int32_t num_blocks,
+    const float* cos_sin, int32_t max_pos, int32_t rot, int32_t interleaved, const void* q_weight, const void* k_weight,
+    int32_t weights_f32, float eps, uint16_t* q_out, int64_t qo_stride_tok, int64_t qo_stride_head, uint16_t* k_out,
+    int64_t ko_stride_tok, int64_t ko_stride_head, int32_t n_tokens, int32_t n_heads, int32_t n_kv, int32_t head_dim,
+    int32_t page, void* stream)
+{
+    const char* what = "locks_kv4_write";
+    QkvArgs a{q, q_stride_tok, q_stride_head, k, k_stride_tok, k_stride_head, v, v_stride_tok, v_stride_head,
+              positions, slot_mapping, nullptr, 0, 0, 0, nullptr, 0, 0, 0, cos_sin, q_weight, k_weight, q_out,
+              qo_stride_tok, qo_stride_head, k_out, ko_stride_tok, ko_stride_head, (long)num_blocks * page, max_pos, rot,
+              n_tokens, n_heads, n_kv, page_shift(page), 0, eps, 0, 0, {}, cache, c_stride_block, c_stride_head};
+    int rc = check_kv4(what, cache, c_stride_block, c_stride_head, num_blocks, n_kv, head_dim, page);
+    if (rc) return rc;
+    rc = check_qkv(what, a, head_dim, page, num_blocks);
+    if (rc) return rc;
+    rc = check_axes(what, a, n_axes, pos_stride_axis, {axes0, axes1, axes2, axes3});
+    if (rc) return rc;
+    return launch_qkv<true>(a, head_dim, interleaved, weights_f32, (hipStream_t)stream);
+}
 
 extern "C" int32_t locks_qkv_write(
     const uint16_t* q, int64_t q_stride_tok, int64_t q_stride_head, const uint16_t* k, int64_t k_stride_tok,
@@ -212,49 +464,12 @@ extern "C" int32_t locks_qkv_write(
     int64_t qo_stride_head, uint16_t* k_out, int64_t ko_stride_tok, int64_t ko_stride_head, int32_t n_tokens,
     int32_t n_heads, int32_t n_kv, int32_t head_dim, int32_t page, void* stream)
 {
-    LOCKS_REQUIRE(head_dim == 64 || head_dim == 128 || head_dim == 256,
-                  "locks_qkv_write: head_dim %d outside {64, 128, 256}", head_dim);
-    LOCKS_REQUIRE(page == 16 || page == 32 || page == 64, "locks_qkv_write: page %d outside {16, 32, 64}", page);
-    LOCKS_REQUIRE(rot >= 0 && rot <= head_dim && rot % 16 == 0,
-                  "locks_qkv_write: rot %d is not a multiple of 16 in [0, head_dim %d]", rot, head_dim);
-    LOCKS_REQUIRE(n_tokens >= 0 && n_heads >= 1 && n_kv >= 1 && num_blocks >= 1 && max_pos >= 1,
-                  "locks_qkv_write: empty geometry");
-    LOCKS_REQUIRE(n_heads <= 4096 && n_kv <= 4096, "locks_qkv_write: more than 4096 heads");
-    LOCKS_REQUIRE(eps >= 0.f, "locks_qkv_write: eps must not be negative");
-    LOCKS_REQUIRE(q && k && v && positions && slot_mapping && k_cache && v_cache && q_out && (cos_sin || rot == 0),
-                  "locks_qkv_write: null pointer argument");
-    for (int64_t x : {q_stride_tok, q_stride_head, k_stride_tok, k_stride_head, v_stride_tok, v_stride_head,
-                      kc_stride_block, kc_stride_tok, kc_stride_head, vc_stride_block, vc_stride_tok, vc_stride_head,
-                      qo_stride_tok, qo_stride_head, ko_stride_tok, ko_stride_head})
-        LOCKS_REQUIRE(x % 8 == 0, "locks_qkv_write: strides must be multiples of 8 elements (16-byte accesses)");
-    for (const void* x : {(const void*)q, (const void*)k, (const void*)v, (const void*)k_cache, (const void*)v_cache,
-                          (const void*)q_out, (const void*)k_out, (const void*)cos_sin, q_weight, k_weight})
-        LOCKS_REQUIRE((uintptr_t)x % 16 == 0, "locks_qkv_write: pointers must be 16-byte aligned");
-    if (n_tokens == 0) return 0;
-    const int per_wave = 512 / head_dim;
-    QkvArgs a{q, q_stride_tok, q_stride_head, k, k_stride_tok, k_stride_head, v, v_stride_tok, v_stride_head,
-              positions, slot_mapping, k_cache, kc_stride_block, kc_stride_tok, kc_stride_head, v_cache,
-              vc_stride_block, vc_stride_tok, vc_stride_head, cos_sin, q_weight, k_weight, q_out, qo_stride_tok,
-              qo_stride_head, k_out, ko_stride_tok, ko_stride_head, (long)num_blocks * page, max_pos, rot,
-              n_tokens, n_heads, n_kv, page == 16 ? 4 : page == 32 ? 5 : 6,
-              cdiv(n_heads + 2 * n_kv, per_wave), eps};
-    hipStream_t st = (hipStream_t)stream;
-    // groups per wave: the angles and weights of a token are loaded once for them,
-    // and their rows are in flight together (8192 tokens of 48 heads: 2 groups 50.5
-    // us, 3 and 4 45)
-    constexpr int IT = 3;
-    const long waves = (long)n_tokens * cdiv(a.groups, IT);
-    const dim3 grid((unsigned)((waves + QK_WAVES - 1) / QK_WAVES));
-#define LAUNCH_W(DV, INTER)                                                                                     \
-    if (weights_f32) hipLaunchKernelGGL((qkv_write_kernel<DV, IT, INTER, true>), grid, dim3(QK_BLK), 0, st, a); \
-    else hipLaunchKernelGGL((qkv_write_kernel<DV, IT, INTER, false>), grid, dim3(QK_BLK), 0, st, a)
-#define LAUNCH(DV)                              \
-    if (interleaved) { LAUNCH_W(DV, true); }    \
-    else { LAUNCH_W(DV, false); }
-    if (head_dim == 64) { LAUNCH(64); }
-    else if (head_dim == 128) { LAUNCH(128); }
-    else { LAUNCH(256); }
-#undef LAUNCH
-#undef LAUNCH_W
-    return check_launch("qkv_write_kernel");
+    const QkvArgs a{q, q_stride_tok, q_stride_head, k, k_stride_tok, k_stride_head, v, v_stride_tok, v_stride_head,
+                    positions, slot_mapping, k_cache, kc_stride_block, kc_stride_tok, kc_stride_head, v_cache,
+                    vc_stride_block, vc_stride_tok, vc_stride_head, cos_sin, q_weight, k_weight, q_out, qo_stride_tok,
+                    qo_stride_head, k_out, ko_stride_tok, ko_stride_head, (long)num_blocks * page, max_pos, rot,
+                    n_tokens, n_heads, n_kv, page_shift(page), 0, eps, 0, 0, {}, nullptr, 0, 0};
+    const int rc = check_qkv("locks_qkv_write", a, head_dim, page, num_blocks);
+    if (rc) return rc;
+    return launch_qkv<false>(a, head_dim, interleaved, weights_f32, (hipStream_t)stream);
 }

@@ -11,7 +11,7 @@ import os
 import struct
 
 _LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_lib", "liblocks_hip.so")
-ABI_VERSION = 11
+ABI_VERSION = 12
 
 _c = ctypes
 _i32, _i64, _f32, _f64, _p = _c.c_int32, _c.c_int64, _c.c_float, _c.c_double, _c.c_void_p
@@ -110,6 +110,21 @@ SIGNATURES = {
     "locks_prefix_decode": (_i32, [_p, _i64, _i64, _p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _i32, _p,
                                    _i64, _i32, _p, _p, _p, _i32, _p, _i64, _i64, _p, _i64, _p, _i64, _i32,
                                    _i32, _i32, _i32, _i32, _i32, _i32, _f32, _p]),
+    "locks_qkv_write_axes": (_i32, [_p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i32, _i64,
+                                    _i64, _i64, _i64, _p, _p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _i32,
+                                    _p, _i32, _i32, _i32, _p, _p, _i32, _f32, _p, _i64, _i64, _p, _i64,
+                                    _i64, _i32, _i32, _i32, _i32, _i32, _p]),
+    "locks_kv4_write": (_i32, [_p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i32, _i64, _i64,
+                               _i64, _i64, _p, _p, _i64, _i64, _i32, _p, _i32, _i32, _i32, _p, _p, _i32,
+                               _f32, _p, _i64, _i64, _p, _i64, _i64, _i32, _i32, _i32, _i32, _i32, _p]),
+    "locks_kv4_read": (_i32, [_p, _i64, _i64, _i32, _p, _p, _i64, _i64, _p, _i64, _i64, _i32, _i32, _i32,
+                              _i32, _p]),
+    "locks_kv4_decode": (_i32, [_p, _i64, _i64, _p, _i64, _i64, _i32, _p, _i64, _i32, _p, _i32, _i32, _p,
+                                _i64, _i64, _p, _i64, _p, _i64, _i32, _i32, _i32, _i32, _i32, _i32, _f32,
+                                _p]),
+    "locks_kv4_prefill": (_i32, [_p, _i64, _i64, _p, _i64, _i64, _i32, _p, _i64, _i32, _p, _p, _i32, _i32,
+                                 _p, _i64, _i64, _p, _i64, _p, _i64, _i32, _i32, _i32, _i32, _i32, _i32,
+                                 _i32, _f32, _p]),
     "locks_call": (_i32, [_i32, _p, _i32]),
     "locks_decode_merge": (_i32, [_p, _p, _p, _p, _i64, _i32, _p, _i64, _i64, _i32, _i32, _i32,
                                   _i32, _i32, _i32, _i32, _i32, _p]),
@@ -173,7 +188,8 @@ def _words(name: str) -> struct.Struct:
 # entry -> (its number for locks_call, the packer of its arguments)
 _CALLS = {name: (i, _words(name)) for i, name in enumerate((
     "locks_tables_step", "locks_tables_trim", "locks_qkv_write", "locks_window_decode", "locks_window_prefill",
-    "locks_prefix_decode"))}
+    "locks_prefix_decode", "locks_qkv_write_axes", "locks_kv4_write", "locks_kv4_read", "locks_kv4_decode",
+    "locks_kv4_prefill"))}
 
 
 def launch(name: str, index: int, args: tuple) -> None:

@@ -4,7 +4,8 @@ The dense layers that stand between the selected ones: ``window_decode`` (one
 new token per request) and ``window_prefill`` (prompt chunks, mixed batches)
 attend to the last ``window`` tokens and to the first ``sinks`` ones, or to
 everything; ``prefix_decode`` reads the pages that a group of requests shares
-once for the whole group.
+once for the whole group.  The first two also take a cache in 4 bits
+(``locks.attention.kv4``).
 """
 from __future__ import annotations
 
@@ -12,6 +13,7 @@ import torch
 
 from .. import _lib
 from .decode import _kv_args
+from .kv4 import kv4_geometry
 
 
 def attn_workspace(device, *, max_tokens: int, n_kv: int, G: int, head_dim: int, max_reqs: int = None) -> torch.Tensor:
@@ -26,7 +28,7 @@ def attn_workspace(device, *, max_tokens: int, n_kv: int, G: int, head_dim: int,
     return torch.empty(n, dtype=torch.uint8, device=device)
 
 
-_BF16, _I32, _F32 = torch.bfloat16, torch.int32, torch.float32
+_BF16, _I32, _F32, _U8 = torch.bfloat16, torch.int32, torch.float32, torch.uint8
 
 
 def _i32(name: str, t, n: int, index: int) -> None:
@@ -38,12 +40,15 @@ def _i32(name: str, t, n: int, index: int) -> None:
 
 def _refuse(what: str, q, kv_cache, block_table, seq_lens, out, ws, lse, rows: int, n_req: int) -> None:
     """The error of a call that _args does not take."""
-    if kv_cache.dim() != 5 or kv_cache.dtype is not _BF16 or kv_cache.stride(-1) != 1:
-        raise TypeError(f"{what}: kv_cache must be a 5-d bf16 cache with a contiguous last dim, got "
-                        f"{kv_cache.dtype} {tuple(kv_cache.shape)}")
-    _, vp, _, (_, _, n_kv, d) = _kv_args(kv_cache)
-    if vp is None:
-        raise ValueError(f"{what} needs a cache with a V half")
+    if kv_cache.dtype is _U8 and what != "prefix_decode":
+        _, _, n_kv, d = kv4_geometry(what, kv_cache)
+    else:
+        if kv_cache.dim() != 5 or kv_cache.dtype is not _BF16 or kv_cache.stride(-1) != 1:
+            raise TypeError(f"{what}: kv_cache must be a 5-d bf16 cache with a contiguous last dim, got "
+                            f"{kv_cache.dtype} {tuple(kv_cache.shape)}")
+        _, vp, _, (_, _, n_kv, d) = _kv_args(kv_cache)
+        if vp is None:
+            raise ValueError(f"{what} needs a cache with a V half")
     dev = kv_cache.device
     for name, t in (("q", q), ("out", out)):
         if t.dtype is not _BF16 or t.dim() != 3 or t.stride(-1) != 1:
@@ -74,19 +79,27 @@ def _args(what: str, q, kv_cache, block_table, seq_lens, out, ws, lse, rows: int
     """The checks that the calls share (one pass over the tensors' attributes:
     with a message at each check they took 7 us of a small call), and their common
     arguments: of q up to seq_lens; from out to the workspace; n_kv, G, d, page; the
-    device's index."""
+    device's index; whether the cache is one in 4 bits."""
     index = kv_cache.get_device()
+    four = kv_cache.dtype is _U8 and what != "prefix_decode"
     try:
-        n0, n1, page, n_kv, d = kv_cache.shape
-        c0, c1, cst, csh, c4 = kv_cache.stride()
+        if four:
+            NB, n_kv, tiles, rec = kv_cache.shape
+            cb, csh, cst, c4 = kv_cache.stride()
+            page, d = 16 * tiles, rec // 17
+            held = rec % 17 == 0 and cst == rec
+        else:
+            n0, n1, page, n_kv, d = kv_cache.shape
+            c0, c1, cst, csh, c4 = kv_cache.stride()
+            # either cache layout: K and V halves by the first or the second dim
+            first = n0 == 2 and n1 != 2
+            held = kv_cache.dtype is _BF16 and (first or n1 != 1)
         (tq, H, dq), (to, ho, do), (rb, cols), (ts,) = q.shape, out.shape, block_table.shape, seq_lens.shape
         (q0, q1, q2), (o0, o1, o2), (b0, b1), (ss,) = q.stride(), out.stride(), block_table.stride(), seq_lens.stride()
-        # either cache layout: K and V halves by the first or the second dim
-        first = n0 == 2 and n1 != 2
-        ok = (index >= 0 and kv_cache.dtype is _BF16 and q.dtype is _BF16 and out.dtype is _BF16
+        ok = (index >= 0 and held and q.dtype is _BF16 and out.dtype is _BF16
               and block_table.dtype is _I32 and seq_lens.dtype is _I32 and 0 <= rows <= tq and rows <= to
               and 0 <= n_req <= rb and n_req <= ts and H % n_kv == 0 and ho == H and dq == d and do == d and c4 == 1
-              and q2 == 1 and o2 == 1 and b1 == 1 and (ss == 1 or ts < 2) and (first or n1 != 1)
+              and q2 == 1 and o2 == 1 and b1 == 1 and (ss == 1 or ts < 2)
               and q.get_device() == index and out.get_device() == index and block_table.get_device() == index
               and seq_lens.get_device() == index)
         lp = ls = wp = wb = 0
@@ -102,10 +115,13 @@ def _args(what: str, q, kv_cache, block_table, seq_lens, out, ws, lse, rows: int
     if not ok:
         _refuse(what, q, kv_cache, block_table, seq_lens, out, ws, lse, rows, n_req)
     kp = kv_cache.data_ptr()
-    cb = c1 if first else c0
-    head = (q.data_ptr(), q0, q1, kp, cb, cst, csh, kp + 2 * (c0 if first else c1), cb, cst, csh, n1 if first else n0,
-            block_table.data_ptr(), b0, cols, seq_lens.data_ptr())
-    return head, (out.data_ptr(), o0, o1, lp, ls, wp, wb), (n_kv, H // n_kv, d, page), index
+    if four:
+        head = (q.data_ptr(), q0, q1, kp, cb, csh, NB, block_table.data_ptr(), b0, cols, seq_lens.data_ptr())
+    else:
+        cb = c1 if first else c0
+        head = (q.data_ptr(), q0, q1, kp, cb, cst, csh, kp + 2 * (c0 if first else c1), cb, cst, csh,
+                n1 if first else n0, block_table.data_ptr(), b0, cols, seq_lens.data_ptr())
+    return head, (out.data_ptr(), o0, o1, lp, ls, wp, wb), (n_kv, H // n_kv, d, page), index, four
 
 
 def window_decode(q, kv_cache, block_table, seq_lens, out, ws, *, n_req: int, scale: float, window: int = 0,
@@ -117,11 +133,12 @@ def window_decode(q, kv_cache, block_table, seq_lens, out, ws, *, n_req: int, sc
     reads and writes row r: padding takes a row here, though no token in
     ``BlockTables.step``, and so stands behind the requests.  A request of length 0
     (padding) gives zeros and -inf.  ``max_seq_len``: an upper bound of
-    the lengths, where one is known, sizes the launch.  ``ws``: attn_workspace."""
-    head, tail, geo, index = _args("window_decode", q, kv_cache, block_table, seq_lens, out, ws, lse, n_req, n_req)
+    the lengths, where one is known, sizes the launch.  ``ws``: attn_workspace.
+    ``kv_cache``: the paged cache in bf16, or one in 4 bits (``kv4_cache``)."""
+    head, tail, geo, index, four = _args("window_decode", q, kv_cache, block_table, seq_lens, out, ws, lse, n_req, n_req)
     if n_req == 0:
         return
-    _lib.launch("locks_window_decode", index,
+    _lib.launch("locks_kv4_decode" if four else "locks_window_decode", index,
                 (*head, window, sinks, *tail, n_req, *geo, max_seq_len, scale))
 
 
@@ -131,13 +148,14 @@ def window_prefill(q, kv_cache, block_table, seq_lens, query_start_loc, out, ws,
     are the last tokens of request r, whose K and V are in the cache; each sees
     the keys up to its own position, in the window or among the first ``sinks`` as
     for ``window_decode``.  Rows from ``query_start_loc[n_req]`` on stay as they
-    were.  ``n_tokens`` (default: the rows of q) bounds the rows read."""
+    were.  ``n_tokens`` (default: the rows of q) bounds the rows read.  ``kv_cache``
+    as for ``window_decode``."""
     n_tokens = q.shape[0] if n_tokens is None else n_tokens
-    head, tail, geo, index = _args("window_prefill", q, kv_cache, block_table, seq_lens, out, ws, lse, n_tokens, n_req)
+    head, tail, geo, index, four = _args("window_prefill", q, kv_cache, block_table, seq_lens, out, ws, lse, n_tokens, n_req)
     _i32("window_prefill: query_start_loc", query_start_loc, n_req + 1, index)
     if n_req == 0 or n_tokens == 0:
         return
-    _lib.launch("locks_window_prefill", index,
+    _lib.launch("locks_kv4_prefill" if four else "locks_window_prefill", index,
                 (*head, query_start_loc.data_ptr(), window, sinks, *tail, n_tokens, n_req, *geo, max_seq_len, scale))
 
 
@@ -151,7 +169,7 @@ def prefix_decode(q, kv_cache, block_table, seq_lens, group_start, prefix_pages,
     groups, members shorter than the prefix and padding (length 0) are attended
     like any other; their rows need hold no more pages than their lengths.
     ``n_groups`` is at least 1; a group may hold no request."""
-    head, tail, geo, index = _args("prefix_decode", q, kv_cache, block_table, seq_lens, out, ws, lse, n_req, n_req)
+    head, tail, geo, index, _ = _args("prefix_decode", q, kv_cache, block_table, seq_lens, out, ws, lse, n_req, n_req)
     _i32("prefix_decode: group_start", group_start, n_groups + 1, index)
     _i32("prefix_decode: prefix_pages", prefix_pages, n_groups, index)
     if n_req == 0:

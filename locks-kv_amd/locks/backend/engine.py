@@ -25,7 +25,8 @@ integration spreads this over:
   ``block_tables`` (the step's tables and slots from the requests' lengths),
   ``write_qkv`` (norm, rotation and cache write of a layer's projection),
   ``forward_dense`` (prompt chunks and mixed batches, and layers that keep a
-  window) and ``forward_prefix`` (decode of requests on a shared prefix).
+  window) and ``forward_prefix`` (decode of requests on a shared prefix).  Layers
+  that only ever attend densely may hold their cache in 4 bits (``kv4_cache``).
 
 A vLLM-ROCm attention backend calls ``prologue`` from its metadata builder
 and ``forward`` from its impl; any other engine can drive it directly.
@@ -34,7 +35,7 @@ from __future__ import annotations
 
 import torch
 
-from ..attention import attn_workspace, prefix_decode, qk_norm_rope_write, window_decode, window_prefill
+from ..attention import attn_workspace, kv4_cache, prefix_decode, qk_norm_rope_write, window_decode, window_prefill
 from ..attention.decode import _split_kv, ensure_stage_b_buffers
 from ..selection import Rki4State, derive_page_params
 from ..tier import Tier
@@ -135,19 +136,35 @@ class LocksEngine:
                            max_reqs=self.st.max_reqs, max_pages=self.st.max_pages, max_tokens=self.max_tokens,
                            reserved=reserved)
 
+    def kv4_cache(self) -> torch.Tensor:
+        """A cache in 4 bits of this engine's geometry, for a layer outside
+        ``kv_caches`` that ``write_qkv`` and ``forward_dense`` get it for: the same block
+        ids and slots hold for it."""
+        st = self.st
+        return kv4_cache(st.NB, n_kv=st.n_kv, head_dim=st.D, page=st.page, device=self.kv_caches[0].device)
+
     @torch.no_grad()
     def write_qkv(self, layer: int, q, k, v, positions, slot_mapping, cos_sin, q_out, *, n_tokens: int = None,
-                  q_weight=None, k_weight=None, eps: float = 1e-6, interleaved: bool = False) -> None:
+                  q_weight=None, k_weight=None, eps: float = 1e-6, interleaved: bool = False, axes=None,
+                  kv_cache=None) -> None:
         """A layer's projection made ready (``qk_norm_rope_write``): queries to
         ``q_out``, keys and values to the layer's cache and, for the mem variants,
         V (mem-kv: and the keys) to the tier's staging pool (``write_kv``).  This
         and the dense calls need a cache with both halves: a K-only one, which the
-        mem variants' ``forward`` takes too, is refused."""
+        mem variants' ``forward`` takes too, is refused.  ``axes``: the axis of each
+        pair, where positions have several (``RopeAxes``).  ``kv_cache``: the cache of a
+        layer outside ``kv_caches`` (bf16, or ``kv4_cache``), which has no part in
+        selection and tier; ``layer`` does not matter then."""
         n = int(q.shape[0] if n_tokens is None else n_tokens)
+        if kv_cache is not None:
+            qk_norm_rope_write(q, k, v, positions, slot_mapping, kv_cache, cos_sin, q_out, n_tokens=n, q_weight=q_weight,
+                               k_weight=k_weight, eps=eps, interleaved=interleaved, axes=axes)
+            return
         if self.tier is not None and n > self.max_tokens:
             raise ValueError(f"write_qkv: {n} tokens > max_num_batched_tokens {self.max_tokens}")
         qk_norm_rope_write(q, k, v, positions, slot_mapping, self.kv_caches[layer], cos_sin, q_out, n_tokens=n,
-                           q_weight=q_weight, k_weight=k_weight, eps=eps, interleaved=interleaved, k_out=self._k_out)
+                           q_weight=q_weight, k_weight=k_weight, eps=eps, interleaved=interleaved, k_out=self._k_out,
+                           axes=axes)
         if self.tier is not None and n:
             self.write_kv(layer, None if self._k_out is None else self._k_out[:n], v[:n])
 
@@ -165,7 +182,8 @@ class LocksEngine:
                       query_start_loc=None, n_decode: int = None, n_tokens: int = None, window: int = 0, sinks: int = 0,
                       lse=None) -> None:
         """One layer of any step with attention over the whole row, or over the
-        last ``window`` tokens and the first ``sinks``, read from the paged cache.
+        last ``window`` tokens and the first ``sinks``, read from the paged cache (in
+        bf16 or in 4 bits).
         The first ``n_decode`` requests have one new token each, in rows 0 to
         ``n_decode`` - 1 (default: all, without ``query_start_loc``; none with it),
         the others the rows that ``query_start_loc`` gives.  Padding takes no
