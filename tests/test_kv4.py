@@ -101,6 +101,29 @@ def test_write_axes_and_gaps(d, axes, w):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("T", [9, 700])
+def test_write_where_fp32_would_not_do(T, interleaved):
+    """Weights past 2^60, sums of squares that overflow fp32 or underflow, rows whose entries
+    cancel: the codes are those of 64 bits all the same."""
+    x = inputs(T, 8, 4, 128, 128, 1, w=torch.float32, seed=T)
+    x["kw"][5], x["kw"][70] = 1e30, -1e19
+    x["k"][0], x["k"][1] = x["k"][0] * 1e30, x["k"][1] * 1e-30
+    x["k"][2, :, :64] = x["k"][2, :, 64:]
+    x["q"][0] = 0
+    x["pos"][0, 0:2] = 3
+    cache = _blank(x["blocks"], 4, 128, 16)
+    q = torch.zeros_like(x["q"])
+    for kw in (x["kw"], torch.ones_like(x["kw"])):
+        qk_norm_rope_write(x["q"], x["k"], x["v"], x["pos"][0], x["slots"], cache, x["cs"], q, q_weight=x["qw"],
+                           k_weight=kw, interleaved=interleaved)
+        k64 = formula(x["k"], kw, x["pos"], x["cs"], RopeAxes([0] * 64), float(torch.tensor(1e-6)), interleaved)[0]
+        _, _, want, near = quantised(k64)
+        k, _ = _read(cache, x["slots"])
+        assert torch.equal(torch.where(near, 0, k.double()), torch.where(near, 0, want)) and int(near.sum()) < 3
+
+
+@pytest.mark.gpu
 def test_write_many_tokens():
     x = inputs(5000, 3, 1, 128, 128, 1, page=16)
     _written(x, None, _blank(x["blocks"], 1, 128, 16))
