@@ -68,7 +68,7 @@ int32_t check_ws(const char* what, const void* ws, int64_t have, int64_t need);
 int32_t check_kv4(const char* what, const void* cache, int64_t sb, int64_t sh, int32_t num_blocks, int32_t n_kv,
                   int32_t head_dim, int32_t page);
 
-// Workgroups of a row of a single-token call on a cache in 4 bits (locks_kv4.hip).
-int kv4_decode_splits(int n_req, int n_kv, long max_keys);
+// Workspace of a single-token call on one (locks_kv4.hip).
+int64_t kv4_workspace(int n_req, int n_kv, int G, int head_dim);
 
 }  // namespace locks

@@ -27,6 +27,7 @@
 namespace locks {
 
 typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
+typedef int v2i __attribute__((ext_vector_type(2)));
 
 template <int D>
 struct Kv4 {
@@ -62,13 +63,13 @@ struct Kv4Lane {
 template <int D>
 __device__ __forceinline__ void kv4_codes(const uint8_t* p, int lane, uint32_t* w) {
     if constexpr (D == 64) {
-        const uint2 x = *reinterpret_cast<const uint2*>(p + lane * 8);
-        w[0] = x.x; w[1] = x.y;
+        const v2i x = __builtin_nontemporal_load(reinterpret_cast<const v2i*>(p + lane * 8));
+        w[0] = x[0]; w[1] = x[1];
     } else {
 #pragma unroll
         for (int i = 0; i < D / 128; ++i) {
-            const uint4 x = *reinterpret_cast<const uint4*>(p + i * 1024 + lane * 16);
-            w[4 * i] = x.x; w[4 * i + 1] = x.y; w[4 * i + 2] = x.z; w[4 * i + 3] = x.w;
+            const v4i x = __builtin_nontemporal_load(reinterpret_cast<const v4i*>(p + i * 1024 + lane * 16));
+            w[4 * i] = x[0]; w[4 * i + 1] = x[1]; w[4 * i + 2] = x[2]; w[4 * i + 3] = x[3];
         }
     }
 }

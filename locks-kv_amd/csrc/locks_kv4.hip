@@ -11,7 +11,13 @@
 //   O^T += V^T P^T: a lane's weights are the operand as they stand; its V codes are
 //       four keys of d / 16 entries, which pair up by one byte permutation a pair.
 // Every wave keeps its own running maximum and sum; the waves of a workgroup join in
-// LDS, the workgroups of a row in attn_merge_kernel.
+// LDS, and the workgroups of a row in kv4_merge_kernel.
+//
+// Work is dealt out in equal shares (bound by memory, a call is as long as its longest
+// workgroup, and lengths are known to the GPU alone): the tiles of all (request, kv
+// head) rows in order, K4_ROW tiles' worth more for each row's start, cut into one share
+// a workgroup.  A share holds whole rows, whose outputs it writes, and at most an end of
+// one row and a start of another, whose partials go to its two slots.
 #include "locks_attn.h"
 #include "locks_common.h"
 #include "locks_hip.h"
@@ -19,11 +25,16 @@
 
 #include <math.h>
 
+#include <type_traits>
+
 namespace locks {
 
 constexpr int K4_WAVES = 4;
 constexpr int K4_BLK = K4_WAVES * kWave;
-constexpr float kLog2e = 1.44269504088896340736f;
+constexpr int K4_TILES = 2;                 // of a wave's step
+constexpr int K4_ROW = 32;                  // a row's start (query, first loads, output) in tiles' time
+constexpr int K4_SHARE = 24;                // tiles that a share has at least
+constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 
 struct Kv4DecodeArgs {
     const uint16_t* q; long q_sr, q_sh;
@@ -32,48 +43,150 @@ struct Kv4DecodeArgs {
     const int* seq_lens;
     uint16_t* out; long o_sr, o_sh;
     float* lse; long lse_sr;
-    Partials p;                                     // splits 1: none, the output is written
-    float scale_log2, scale;
-    int NB, bt_cols, n_kv, G, pg_sh, window, sinks, chunk;      // chunk: tiles of a workgroup
+    // partials by slot (two a share) and head of the group, and the shares of each row
+    float* m; float* l; float* acc; int2* shares;
+    float scale_log2;
+    double inv_grid;                                // 1 / workgroups
+    int NB, bt_cols, n_req, n_kv, G, pg_sh, window, sinks;
+    bool rows;                                      // a workgroup for each row: no shares, no partials
 };
+
+// The keys that a request's query sees, as tiles: the first na, then [b0, b0 + nt - na).
+struct Kv4Row {
+    int len, lo, sinks, na, b0, nt;
+    __device__ __forceinline__ Kv4Row(const Kv4DecodeArgs& a, int seq_len) {
+        const long cap = (long)a.bt_cols << a.pg_sh, full = max(seq_len, 0);
+        len = (int)min(full, cap);
+        // (a length past the table: the window still ends at it)
+        lo = a.window ? (int)min(max(full - a.window, 0L), (long)len) : 0;
+        sinks = min(a.sinks, lo);
+        na = (sinks + 15) >> 4;
+        b0 = max(lo >> 4, na);
+        nt = na + max(((len + 15) >> 4) - b0, 0);
+    }
+    __device__ __forceinline__ int cost() const { return K4_ROW + max(nt, 1); }
+};
+
+// A value that every lane holds, in scalar registers.
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ long uniform(long x) {
+    return (long)((uint64_t)(uint32_t)uniform((int)x) | (uint64_t)(uint32_t)uniform((int)(x >> 32)) << 32);
+}
+
+// Inclusive prefix sums over the wave, as wave_incl_scan_i.
+__device__ __forceinline__ double wave_incl_scan(double v) {
+    auto shifted = [](double x, auto ctrl, auto rows) __attribute__((always_inline)) {
+        const long u = __double_as_longlong(x);
+        const int lo = __builtin_amdgcn_update_dpp(0, (int)u, ctrl(), rows(), 0xf, false);
+        const int hi = __builtin_amdgcn_update_dpp(0, (int)(u >> 32), ctrl(), rows(), 0xf, false);
+        return __longlong_as_double((long)((uint64_t)(uint32_t)lo | (uint64_t)(uint32_t)hi << 32));
+    };
+    using All = std::integral_constant<int, 0xf>;
+    v += shifted(v, std::integral_constant<int, 0x111>{}, All{});
+    v += shifted(v, std::integral_constant<int, 0x112>{}, All{});
+    v += shifted(v, std::integral_constant<int, 0x114>{}, All{});
+    v += shifted(v, std::integral_constant<int, 0x118>{}, All{});
+    v += shifted(v, std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xa>{});
+    v += shifted(v, std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xc>{});
+    return v;
+}
 
 // Bits 2 lo .. of two words as one: {low or high halves of a, of b}.
 __device__ __forceinline__ uint32_t lows(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x05040100u); }
 __device__ __forceinline__ uint32_t highs(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
 
 template <int D>
-__global__ __launch_bounds__(K4_BLK, D == 256 ? 2 : 3) void kv4_decode_kernel(const Kv4DecodeArgs a)
+__global__ __launch_bounds__(K4_BLK, 2) void kv4_decode_kernel(const Kv4DecodeArgs a)
 {
     using L = Kv4<D>;
-    constexpr int ND = D / 16, W = L::W;
+    constexpr int ND = D / 16, W = L::W, T = K4_TILES;
     __shared__ float m_s[K4_WAVES][16], l_s[K4_WAVES][16];
     __shared__ __attribute__((aligned(16))) float o_s[K4_WAVES][16][D + 4];
+    __shared__ double sum_s[K4_WAVES];
+    __shared__ long at_s[2];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int c16 = lane & 15, kg = lane >> 4;
-    const int nsplit = a.p.splits, G = a.G;
-    const int sp = blockIdx.x % nsplit, kh = blockIdx.x / nsplit % a.n_kv;
-    const long r = blockIdx.x / nsplit / a.n_kv;
+    const int G = a.G;
 
-    const long cap = (long)a.bt_cols << a.pg_sh;
-    const int len = (int)min((long)max(a.seq_lens[r], 0), cap);
-    // a length past the table: the window still ends at it
-    const long full = max(a.seq_lens[r], 0);
-    const int lo = a.window ? (int)min(max(full - a.window, 0L), (long)len) : 0;
-    const int sinks = min(a.sinks, lo);
-    // tiles: the first na, then [b0, b1); this workgroup's [n0, n1) of them
-    const int na = (sinks + 15) >> 4, b0 = max(lo >> 4, na), b1 = (len + 15) >> 4;
-    const int nt = na + max(b1 - b0, 0);
-    const int n0 = min(sp * a.chunk, nt), n1 = sp == nsplit - 1 ? nt : min(n0 + a.chunk, nt);
-    const long row = (r * a.n_kv + kh) * nsplit + sp;
-    if (n0 >= n1 && nsplit > 1) {
-        if (tid < G) { a.p.m[row * G + tid] = -INFINITY; a.p.l[row * G + tid] = 0.f; }
-        return;
+    // this workgroup's share [lo, hi) of all rows' cost, and the row that it starts in
+    int r = 0, kh = 0;
+    long start = 0, lo = 0, hi = 0, total = 0;      // start: of row (r, kh)
+    long share = 0;
+    if (a.rows) {
+        r = blockIdx.x / a.n_kv;
+        kh = blockIdx.x % a.n_kv;
+        hi = 0x7fffffff;
+    } else {
+        // (sums as doubles: exact up to 2^53, and their quotients' whole parts too)
+        const int sh = blockIdx.x;
+        if (a.n_req <= kWave) {                     // every wave by itself
+            const Kv4Row mine(a, a.seq_lens[min(lane, a.n_req - 1)]);
+            const double cost = lane < a.n_req ? (double)mine.cost() * a.n_kv : 0.0, inc = wave_incl_scan(cost);
+            total = uniform((long)__shfl(inc, 63));
+            share = max((long)((double)total * a.inv_grid) + 1, (long)K4_SHARE);
+            lo = sh * share;
+            if (lo >= total) return;
+            r = __ffsll(__ballot(inc > (double)lo)) - 1;
+            start = uniform((long)__shfl(inc - cost, r));
+        } else {
+            const int per = (a.n_req + K4_BLK - 1) / K4_BLK;       // consecutive requests of a thread
+            const int r0 = min(tid * per, a.n_req), r1 = min(r0 + per, a.n_req);
+            double mine = 0.0;
+            for (int i = r0; i < r1; ++i) mine += (double)Kv4Row(a, a.seq_lens[i]).cost() * a.n_kv;
+            const double inc = wave_incl_scan(mine);
+            if (lane == 63) sum_s[wave] = inc;
+            __syncthreads();
+            double before = inc - mine, all = 0.0;
+            for (int w = 0; w < K4_WAVES; ++w) {
+                before += w < wave ? sum_s[w] : 0.0;
+                all += sum_s[w];
+            }
+            total = uniform((long)all);
+            share = max((long)((double)total * a.inv_grid) + 1, (long)K4_SHARE);
+            lo = sh * share;
+            if (lo >= total) return;
+            if (before <= (double)lo && (double)lo < before + mine) {
+                int i = r0;
+                for (;; ++i) {
+                    const double c = (double)Kv4Row(a, a.seq_lens[i]).cost() * a.n_kv;
+                    if (i == r1 - 1 || (double)lo < before + c) break;
+                    before += c;
+                }
+                at_s[0] = i;
+                at_s[1] = (long)before;
+            }
+            __syncthreads();
+            r = uniform((int)at_s[0]);
+            start = uniform(at_s[1]);
+        }
+        hi = min(lo + share, total);
+        const int c = Kv4Row(a, uniform(a.seq_lens[r])).cost();
+        kh = uniform((int)((double)(lo - start) / (double)c));
+        start += (long)kh * c;
     }
 
+    for (;;) {
+    const Kv4Row row(a, uniform(a.seq_lens[r]));
+    const int len = row.len, klo = row.lo, sinks = row.sinks, na = row.na, b0 = row.b0;
+    const int units = max(row.nt, 1);
+    // the row's tiles [n0, n1) are this share's
+    const long first = start + K4_ROW;
+    int n0 = __builtin_amdgcn_readfirstlane((int)min(max(lo - first, 0L), (long)units));
+    int n1 = __builtin_amdgcn_readfirstlane((int)min(max(hi - first, 0L), (long)units));
+    if (a.rows) { n0 = 0; n1 = units; }
+    const bool whole = n0 == 0 && n1 == units;
+    const bool work = n0 < n1;
+    const long slot = 2L * blockIdx.x + (n0 == 0);
+    if (!a.rows && work && n0 == 0 && tid == 0) {
+        a.shares[(long)r * a.n_kv + kh] =
+            whole ? make_int2(0, -1) : make_int2((int)blockIdx.x, (int)((double)(first + units - 1) / (double)share));
+    }
+    n1 = min(n1, row.nt);
+    if (work) {
     // Q: k-slots 8 kg .. of step st are entries kg D / 4 + 8 st ..
     v8bf qf[W];
     {
-        const uint16_t* qp = a.q + r * a.q_sr + (long)(kh * G + c16) * a.q_sh + kg * (D / 4);
+        const uint16_t* qp = a.q + (long)r * a.q_sr + (long)(kh * G + c16) * a.q_sh + kg * (D / 4);
 #pragma unroll
         for (int st = 0; st < W; ++st) {
             uint4 w = make_uint4(0u, 0u, 0u, 0u);
@@ -82,27 +195,35 @@ __global__ __launch_bounds__(K4_BLK, D == 256 ? 2 : 3) void kv4_decode_kernel(co
         }
     }
 
-    auto tile_of = [&](int n) __attribute__((always_inline)) { return n < na ? n : b0 + n - na; };
-    // step `it` of this wave: tiles n0 + 2 (wave + K4_WAVES it) and the next one; the
-    // block ids of 32 steps are loaded at once
-    const int mine = n0 + 2 * wave;
-    const int steps = n1 > mine ? (n1 - mine + 2 * K4_WAVES - 1) / (2 * K4_WAVES) : 0;
-    const int per = 1 << (a.pg_sh - 4);             // tiles of a page
-    int ids = 0, ids0 = 0;
-    auto fetch_ids = [&](int it) __attribute__((always_inline)) {
-        ids0 = it;
-        const int n = min(mine + 2 * K4_WAVES * (it + (lane >> 1)) + (lane & 1), n1 - 1);
-        const int pg = min(tile_of(n) >> (a.pg_sh - 4), a.bt_cols - 1);
-        ids = min(max(a.bt[r * a.bt_sr + pg], 0), a.NB - 1);
+    // step `it` of this wave: tiles n0 + T (wave + K4_WAVES it) .., T of them.  Addresses
+    // and first keys of 64 tiles are made at once, one per lane.
+    const int mine = n0 + T * wave;
+    const int steps = n1 > mine ? (n1 - mine + T * K4_WAVES - 1) / (T * K4_WAVES) : 0;
+    uint32_t at_lo = 0, at_hi = 0;
+    int key_of = 0, it_of = 0;
+    uint64_t edges = 0;
+    auto fetch = [&](int it) __attribute__((always_inline)) {
+        it_of = it;
+        const int n = mine + T * (K4_WAVES * (it + lane / T)) + lane % T, nc = min(n, n1 - 1);
+        const int tile = nc < na ? nc : b0 + nc - na;
+        const int id = a.bt[(long)r * a.bt_sr + min(tile >> (a.pg_sh - 4), a.bt_cols - 1)];
+        const uint64_t at = (uint64_t)a.c + (uint64_t)((long)min(max(id, 0), a.NB - 1) * a.c_sb + (long)kh * a.c_sh +
+                                                       (tile & ((1 << (a.pg_sh - 4)) - 1)) * L::TILE);
+        at_lo = (uint32_t)at;
+        at_hi = (uint32_t)(at >> 32);
+        key_of = n < n1 ? tile << 4 : 0x7fffffc0;   // behind the share: keys that no query sees
+        edges = __ballot(key_of + 15 >= len || !(key_of >= klo || key_of + 16 <= sinks));
     };
-    struct Step { Kv4Lane<D> k[2], v[2]; };
+    struct Step { Kv4Lane<D> k[T], v[T]; int key0[T]; bool edge; };
     auto load = [&](int it, Step& x) __attribute__((always_inline)) {
-        if (it - ids0 >= 32) fetch_ids(it);
+        if (it - it_of >= kWave / T) fetch(it);
+        const int l0 = T * (it - it_of);
+        x.edge = (edges >> l0 & ((1u << T) - 1)) != 0;
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            const int n = min(mine + 2 * K4_WAVES * it + t, n1 - 1);
-            const long blk = __builtin_amdgcn_readlane(ids, 2 * (it - ids0) + t);
-            const uint8_t* p = a.c + blk * a.c_sb + (long)kh * a.c_sh + (tile_of(n) & (per - 1)) * L::TILE;
+        for (int t = 0; t < T; ++t) {
+            const uint8_t* p = reinterpret_cast<const uint8_t*>((uint64_t)(uint32_t)__builtin_amdgcn_readlane(at_lo, l0 + t) |
+                                                                (uint64_t)(uint32_t)__builtin_amdgcn_readlane(at_hi, l0 + t) << 32);
+            x.key0[t] = __builtin_amdgcn_readlane(key_of, l0 + t);
             kv4_load_k<D>(p, lane, x.k[t]);
             kv4_load_v<D>(p, lane, x.v[t]);
         }
@@ -113,10 +234,10 @@ __global__ __launch_bounds__(K4_BLK, D == 256 ? 2 : 3) void kv4_decode_kernel(co
 #pragma unroll
     for (int b = 0; b < ND; ++b) o[b] = v4f{0.f, 0.f, 0.f, 0.f};
 
-    auto compute = [&](int it, Step& x) __attribute__((always_inline)) {
-        v4f s[2];
+    auto compute = [&](Step& x) __attribute__((always_inline)) {
+        v4f s[T];
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
+        for (int t = 0; t < T; ++t) {
             s[t] = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int st = 0; st < W; ++st) {
@@ -126,28 +247,24 @@ __global__ __launch_bounds__(K4_BLK, D == 256 ? 2 : 3) void kv4_decode_kernel(co
             }
         }
         // keys that the query does not see: no weight, and no value (0 x NaN)
+        if (x.edge) {
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            const int n = mine + 2 * K4_WAVES * it + t, key0 = tile_of(n) << 4;
-            const bool whole = n < n1 && key0 + 16 <= len && (key0 >= lo || key0 + 16 <= sinks);
-            if (!whole) {
+            for (int t = 0; t < T; ++t)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const int key = key0 + 4 * kg + i;
-                    const bool seen = n < n1 && key < len && (key >= lo || key < sinks);
+                    const int key = x.key0[t] + 4 * kg + i;
+                    const bool seen = key < len && (key >= klo || key < sinks);
                     s[t][i] = seen ? s[t][i] : -INFINITY;
-                    if (!seen) {
-                        x.v[t].s &= ~(255u << (8 * i));
-                        if constexpr (D == 64) x.v[t].w[i >> 1] &= (i & 1) ? 0xFFFFu : 0xFFFF0000u;
-                        else if constexpr (D == 128) x.v[t].w[i] = 0;
-                        else { x.v[t].w[2 * i] = 0; x.v[t].w[2 * i + 1] = 0; }
-                    }
+                    x.v[t].s &= seen ? ~0u : ~(255u << (8 * i));
+                    if constexpr (D == 64) x.v[t].w[i >> 1] &= seen ? ~0u : (i & 1) ? 0xFFFFu : 0xFFFF0000u;
+                    else
+#pragma unroll
+                        for (int j = 0; j < D / 128; ++j) x.v[t].w[i * (D / 128) + j] &= seen ? ~0u : 0u;
                 }
-            }
         }
         float mx = s[0][0];
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < T; ++t)
 #pragma unroll
             for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[t][i]);
         mx = xor32_max(xor16_max(mx));
@@ -155,8 +272,7 @@ __global__ __launch_bounds__(K4_BLK, D == 256 ? 2 : 3) void kv4_decode_kernel(co
         // are at most 256, and o and l need no rescaling
         if (__any((mx - m) * a.scale_log2 > 8.f)) {
             const float m_new = fmaxf(m, mx);
-            const float alpha = __builtin_amdgcn_exp2f((m - m_new) * a.scale_log2);
-            const float al = m_new == -INFINITY ? 1.f : alpha;
+            const float al = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - m_new) * a.scale_log2);
             m = m_new;
             l *= al;
 #pragma unroll
@@ -165,62 +281,65 @@ __global__ __launch_bounds__(K4_BLK, D == 256 ? 2 : 3) void kv4_decode_kernel(co
         const float mc = m == -INFINITY ? 0.f : m * a.scale_log2;
         // Weights in bf16, the product's other operand (half a step, 2^-8 of each);
         // l keeps the unrounded ones
-        v8bf pf;
+        v8bf pf[T / 2];
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < T; ++t)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const float p = __builtin_amdgcn_exp2f(fmaf(s[t][i], a.scale_log2, -mc));
                 l += p;
-                pf[4 * t + i] = (__bf16)p;
+                pf[t >> 1][4 * (t & 1) + i] = (__bf16)p;
             }
-        float vs[2][4];
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) vs[t][i] = kv4_scale(x.v[t].s, i);
-        // two column blocks at once: the entries 2 j and 2 j + 1 of every lane's share
-        auto pair = [&](auto byte, int b, int word, int step) __attribute__((always_inline)) {
-            constexpr int B = decltype(byte)::value;
-            uint32_t y[2][4];
+        for (int u = 0; u < T / 2; ++u) {
+            const Kv4Lane<D>* v = x.v + 2 * u;
+            float vs[2][4];
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if constexpr (D == 64) {
-                        y[t][i] = (i & 1) ? kv4_pair<B + 2>(x.v[t].w[i >> 1], vs[t][i]) : kv4_pair<B>(x.v[t].w[i >> 1], vs[t][i]);
-                    } else {
-                        y[t][i] = kv4_pair<B>(x.v[t].w[step * i + word], vs[t][i]);
-                    }
-                }
-            const uint4 even = make_uint4(lows(y[0][0], y[0][1]), lows(y[0][2], y[0][3]), lows(y[1][0], y[1][1]), lows(y[1][2], y[1][3]));
-            const uint4 odd = make_uint4(highs(y[0][0], y[0][1]), highs(y[0][2], y[0][3]), highs(y[1][0], y[1][1]), highs(y[1][2], y[1][3]));
-            o[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, even), pf, o[b], 0, 0, 0);
-            o[b + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, odd), pf, o[b + 1], 0, 0, 0);
-        };
-        using B0 = std::integral_constant<int, 0>; using B1 = std::integral_constant<int, 1>;
-        using B2 = std::integral_constant<int, 2>; using B3 = std::integral_constant<int, 3>;
-        if constexpr (D == 64) {
-            pair(B0{}, 0, 0, 0); pair(B1{}, 2, 0, 0);
-        } else {
+                for (int i = 0; i < 4; ++i) vs[t][i] = kv4_scale(v[t].s, i);
+            // two column blocks at once: the entries 2 j and 2 j + 1 of every lane's share
+            auto pair = [&](auto byte, int b, int word) __attribute__((always_inline)) {
+                constexpr int B = decltype(byte)::value;
+                uint32_t y[2][4];
 #pragma unroll
-            for (int w = 0; w < D / 128; ++w) {
-                pair(B0{}, 8 * w, w, D / 128); pair(B1{}, 8 * w + 2, w, D / 128);
-                pair(B2{}, 8 * w + 4, w, D / 128); pair(B3{}, 8 * w + 6, w, D / 128);
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        if constexpr (D == 64)
+                            y[t][i] = (i & 1) ? kv4_pair<(B + 2) & 3>(v[t].w[i >> 1], vs[t][i]) : kv4_pair<B>(v[t].w[i >> 1], vs[t][i]);
+                        else
+                            y[t][i] = kv4_pair<B>(v[t].w[(D / 128) * i + word], vs[t][i]);
+                    }
+                const uint4 even = make_uint4(lows(y[0][0], y[0][1]), lows(y[0][2], y[0][3]), lows(y[1][0], y[1][1]), lows(y[1][2], y[1][3]));
+                const uint4 odd = make_uint4(highs(y[0][0], y[0][1]), highs(y[0][2], y[0][3]), highs(y[1][0], y[1][1]), highs(y[1][2], y[1][3]));
+                o[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, even), pf[u], o[b], 0, 0, 0);
+                o[b + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, odd), pf[u], o[b + 1], 0, 0, 0);
+            };
+            using B0 = std::integral_constant<int, 0>; using B1 = std::integral_constant<int, 1>;
+            using B2 = std::integral_constant<int, 2>; using B3 = std::integral_constant<int, 3>;
+            if constexpr (D == 64) {
+                pair(B0{}, 0, 0); pair(B1{}, 2, 0);
+            } else {
+#pragma unroll
+                for (int w = 0; w < D / 128; ++w) {
+                    pair(B0{}, 8 * w, w); pair(B1{}, 8 * w + 2, w);
+                    pair(B2{}, 8 * w + 4, w); pair(B3{}, 8 * w + 6, w);
+                }
             }
         }
     };
 
     if (steps > 0) {
-        Step x0, x1;
-        fetch_ids(0);
+        Step x0, x1;                                // the one in use and the one on its way
+        fetch(0);
         load(0, x0);
         for (int it = 0; it < steps; it += 2) {
             if (it + 1 < steps) load(it + 1, x1);
-            compute(it, x0);
+            compute(x0);
             if (it + 1 < steps) {
                 if (it + 2 < steps) load(it + 2, x0);
-                compute(it + 1, x1);
+                compute(x1);
             }
         }
     }
@@ -253,18 +372,106 @@ __global__ __launch_bounds__(K4_BLK, D == 256 ? 2 : 3) void kv4_decode_kernel(co
             lt += lw * f;
             acc.x += f * y.x; acc.y += f * y.y; acc.z += f * y.z; acc.w += f * y.w;
         }
-        constexpr float kLn2 = 0.69314718055994530942f;
-        if (nsplit > 1) {
-            *reinterpret_cast<float4*>(a.p.acc + (row * G + g) * D + e) = acc;
-            if (e == 0) { a.p.m[row * G + g] = mm * kLn2; a.p.l[row * G + g] = lt; }
+        if (!whole) {
+            *reinterpret_cast<float4*>(a.acc + (slot * G + g) * D + e) = acc;
+            if (e == 0) { a.m[slot * G + g] = mm; a.l[slot * G + g] = lt; }
         } else {
             const float inv = lt == 0.f ? 0.f : 1.f / lt;
             uint2 w;
             w.x = (uint32_t)f32_to_bf16(acc.x * inv) | (uint32_t)f32_to_bf16(acc.y * inv) << 16;
             w.y = (uint32_t)f32_to_bf16(acc.z * inv) | (uint32_t)f32_to_bf16(acc.w * inv) << 16;
-            *reinterpret_cast<uint2*>(a.out + r * a.o_sr + (long)(kh * G + g) * a.o_sh + e) = w;
-            if (a.lse && e == 0) a.lse[r * a.lse_sr + kh * G + g] = lt == 0.f ? -INFINITY : mm * kLn2 + logf(lt);
+            *reinterpret_cast<uint2*>(a.out + (long)r * a.o_sr + (long)(kh * G + g) * a.o_sh + e) = w;
+            if (a.lse && e == 0) a.lse[(long)r * a.lse_sr + kh * G + g] = lt == 0.f ? -INFINITY : mm * kLn2 + logf(lt);
         }
+    }
+    __syncthreads();
+    }
+    // the next row
+    start += row.cost();
+    if (a.rows || start >= hi) break;
+    if (++kh == a.n_kv) { kh = 0; ++r; }
+    }
+}
+
+// Joins the shares of every row that has several: one workgroup per (request, head),
+// D / 4 columns of K4_BLK 4 / D streams over the shares.  The first share's partial is in
+// its second slot (it starts the row), the others' in their first.
+constexpr int K4_GRID = 512;                // shares at most: two workgroups a CU
+template <int D>
+__global__ __launch_bounds__(K4_BLK) void kv4_merge_kernel(const Kv4DecodeArgs a)
+{
+    constexpr int COLS = D / 4, STREAMS = K4_BLK / COLS, PF = 8;
+    __shared__ float w_s[K4_GRID];
+    __shared__ float4 part[STREAMS][COLS];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int col = tid % COLS, strm = tid / COLS;
+    const int H = a.n_kv * a.G, hd = blockIdx.x % H, kh = hd / a.G, g = hd % a.G;
+    const long r = blockIdx.x / H;
+    const int2 sh = a.shares[r * a.n_kv + kh];
+    const int n = sh.y - sh.x + 1;
+    if (n <= 0) return;
+    auto at = [&](int i) __attribute__((always_inline)) { return (2L * (sh.x + i) + (i == 0)) * a.G + g; };
+    // every load that needs no other goes out first; each wave makes all weights
+    float4 pre[PF];
+#pragma unroll
+    for (int k = 0; k < PF; ++k)
+        pre[k] = *reinterpret_cast<const float4*>(a.acc + at(min(strm + k * STREAMS, n - 1)) * D + 4 * col);
+    constexpr int NK = K4_GRID / kWave;
+    float ms[NK], ls[NK], mm = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < NK; ++k) {
+        if (k * kWave >= n) break;
+        const int i = lane + k * kWave;
+        ls[k] = i < n ? a.l[at(i)] : 0.f;
+        ms[k] = i < n ? a.m[at(i)] : -INFINITY;
+        if (ls[k] == 0.f) ms[k] = -INFINITY;
+        mm = fmaxf(mm, ms[k]);
+    }
+    mm = wave_max(mm);
+    float lt = 0.f;
+#pragma unroll
+    for (int k = 0; k < NK; ++k) {
+        if (k * kWave >= n) break;
+        const int i = lane + k * kWave;
+        const float w = ls[k] == 0.f ? 0.f : mm == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ms[k] - mm);
+        lt += ls[k] * w;
+        if (tid < kWave && i < n) w_s[i] = w;
+    }
+    lt = wave_sum(lt);
+    __syncthreads();
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto add = [&](float w, const float4& x) __attribute__((always_inline)) {
+        if (w != 0.f) { acc.x += w * x.x; acc.y += w * x.y; acc.z += w * x.z; acc.w += w * x.w; }
+    };
+#pragma unroll
+    for (int k = 0; k < PF; ++k) {
+        const int i = strm + k * STREAMS;
+        if (i < n) add(w_s[i], pre[k]);
+    }
+    for (int i0 = strm + PF * STREAMS; i0 < n; i0 += PF * STREAMS) {
+#pragma unroll
+        for (int k = 0; k < PF; ++k)
+            pre[k] = *reinterpret_cast<const float4*>(a.acc + at(min(i0 + k * STREAMS, n - 1)) * D + 4 * col);
+#pragma unroll
+        for (int k = 0; k < PF; ++k) {
+            const int i = i0 + k * STREAMS;
+            if (i < n) add(w_s[i], pre[k]);
+        }
+    }
+    part[strm][col] = acc;
+    __syncthreads();
+    if (tid < COLS) {
+#pragma unroll
+        for (int k = 1; k < STREAMS; ++k) {
+            const float4 x = part[k][tid];
+            acc.x += x.x; acc.y += x.y; acc.z += x.z; acc.w += x.w;
+        }
+        const float inv = lt == 0.f ? 0.f : 1.f / lt;
+        uint2 w;
+        w.x = (uint32_t)f32_to_bf16(acc.x * inv) | (uint32_t)f32_to_bf16(acc.y * inv) << 16;
+        w.y = (uint32_t)f32_to_bf16(acc.z * inv) | (uint32_t)f32_to_bf16(acc.w * inv) << 16;
+        *reinterpret_cast<uint2*>(a.out + r * a.o_sr + (long)hd * a.o_sh + 4 * tid) = w;
+        if (a.lse && tid == 0) a.lse[r * a.lse_sr + hd] = lt == 0.f ? -INFINITY : mm * kLn2 + logf(lt);
     }
 }
 
@@ -304,15 +511,11 @@ __global__ __launch_bounds__(256) void kv4_read_kernel(const Kv4ReadArgs a)
     *reinterpret_cast<uint4*>(a.v + t * a.v_st + (long)kh * a.v_sh + 8 * l) = kv4_eight(vw, vs);
 }
 
-// Workgroups of a row: about 1024 in all, and each of at most 2048 keys up to 4096
-// workgroups; at least 256 keys each (two steps a wave).
-int kv4_decode_splits(int n_req, int n_kv, long max_keys) {
-    const long rows = (long)n_req * n_kv;
-    const long fill = (1024 + rows - 1) / rows, cap = (4096 + rows - 1) / rows;
-    const long even = (max_keys + 2047) / 2048 < cap ? (max_keys + 2047) / 2048 : cap, least = (max_keys + 255) / 256;
-    long n = fill > even ? fill : even;
-    n = n < least ? n : least;
-    return (int)(n < 1 ? 1 : n > AT_MAX_SPLITS ? AT_MAX_SPLITS : n);
+// Workgroups of a call: one for each row where rows are short, or else as many shares as
+// the card holds at once.
+static bool kv4_rows(int n_req, int n_kv, long max_keys) { return max_keys <= 512; }
+int64_t kv4_workspace(int n_req, int n_kv, int G, int head_dim) {
+    return (int64_t)K4_GRID * 2 * G * (head_dim + 2) * 4 + (int64_t)n_req * n_kv * 8;
 }
 
 int32_t check_kv4(const char* what, const void* cache, int64_t sb, int64_t sh, int32_t num_blocks, int32_t n_kv,
@@ -351,29 +554,34 @@ extern "C" int32_t locks_kv4_decode(
     long keys = (long)bt_cols * page;
     if (max_seq_len > 0 && max_seq_len < keys) keys = max_seq_len;
     if (window && (long)window + sinks + 32 < keys) keys = (long)window + sinks + 32;
-    const int ns = kv4_decode_splits(n_req, n_kv, keys);
-    const int64_t rows = (int64_t)n_req * n_kv * G;
-    Partials p{nullptr, nullptr, nullptr, 1};
-    if (ns > 1) {
-        rc = check_ws(what, workspace, workspace_bytes, part_bytes(rows, ns, head_dim));
+    Kv4DecodeArgs a{q, q_stride_req, q_stride_head, cache, c_stride_block, c_stride_head, block_table, bt_stride, seq_lens,
+                    out, out_stride_req, out_stride_head, lse, lse_stride_req, nullptr, nullptr, nullptr, nullptr,
+                    scale * kLog2e, 1.0 / K4_GRID, num_blocks, bt_cols, n_req, n_kv, G, page == 16 ? 4 : page == 32 ? 5 : 6, window, sinks,
+                    kv4_rows(n_req, n_kv, keys)};
+    int wgs = n_req * n_kv;
+    if (!a.rows) {
+        rc = check_ws(what, workspace, workspace_bytes, kv4_workspace(n_req, n_kv, G, head_dim));
         if (rc) return rc;
-        p = part_layout(workspace, rows, ns, head_dim);
+        wgs = K4_GRID;
+        const int64_t slots = 2L * wgs * G;
+        a.acc = static_cast<float*>(workspace);
+        a.m = a.acc + slots * head_dim;
+        a.l = a.m + slots;
+        a.shares = reinterpret_cast<int2*>(a.l + slots);
     }
-    // tiles of a workgroup: a whole number of steps of its waves.  A window's and the
-    // sinks' tiles stand at any offset, a tile more than their keys fill each.
-    const long wg = 2 * K4_WAVES, tiles = (keys + 15) / 16 + (window ? 2 : 0);
-    const long chunk = ((tiles + ns - 1) / ns + wg - 1) / wg * wg;
-    const Kv4DecodeArgs a{q, q_stride_req, q_stride_head, cache, c_stride_block, c_stride_head, block_table, bt_stride,
-                          seq_lens, out, out_stride_req, out_stride_head, lse, lse_stride_req, p, scale * kLog2e, scale,
-                          num_blocks, bt_cols, n_kv, G, page == 16 ? 4 : page == 32 ? 5 : 6, window, sinks, (int)chunk};
     hipStream_t st = (hipStream_t)stream;
-    const dim3 grid((unsigned)((int64_t)n_req * n_kv * ns));
-    if (head_dim == 64) hipLaunchKernelGGL(kv4_decode_kernel<64>, grid, dim3(K4_BLK), 0, st, a);
-    else if (head_dim == 128) hipLaunchKernelGGL(kv4_decode_kernel<128>, grid, dim3(K4_BLK), 0, st, a);
-    else hipLaunchKernelGGL(kv4_decode_kernel<256>, grid, dim3(K4_BLK), 0, st, a);
+#define KV4_LAUNCH(KERNEL, grid)                                                                                  \
+    do {                                                                                                          \
+        if (head_dim == 64) hipLaunchKernelGGL(KERNEL<64>, dim3((unsigned)(grid)), dim3(K4_BLK), 0, st, a);       \
+        else if (head_dim == 128) hipLaunchKernelGGL(KERNEL<128>, dim3((unsigned)(grid)), dim3(K4_BLK), 0, st, a); \
+        else hipLaunchKernelGGL(KERNEL<256>, dim3((unsigned)(grid)), dim3(K4_BLK), 0, st, a);                     \
+    } while (0)
+    KV4_LAUNCH(kv4_decode_kernel, wgs);
     rc = check_launch("kv4_decode_kernel");
-    if (rc || ns == 1) return rc;
-    return launch_merge(p, out, out_stride_req, out_stride_head, lse, lse_stride_req, n_req, n_kv, G, head_dim, nullptr, 0, st);
+    if (rc || a.rows) return rc;
+    KV4_LAUNCH(kv4_merge_kernel, (int64_t)n_req * n_kv * G);
+#undef KV4_LAUNCH
+    return check_launch("kv4_merge_kernel");
 }
 
 extern "C" int32_t locks_kv4_read(

@@ -787,14 +787,13 @@ extern "C" int64_t locks_attn_workspace_bytes(int32_t max_reqs, int32_t max_toke
         const int shr = shared_splits(prefill_tiles(n, 1, G), n_kv, long_row, head_dim);
         const int64_t b = part_bytes((int64_t)n * n_kv * G, own + shr, head_dim);
         most = b > most ? b : most;
-        const int64_t four = part_bytes((int64_t)n * n_kv * G, kv4_decode_splits(n, n_kv, long_row), head_dim);
-        most = four > most ? four : most;
     }
     for (int n = 1; n <= max_tokens && prefill_tiles(n, 1, G) * n_kv < 256; ++n) {
         const int64_t b = part_bytes((int64_t)n * n_kv * G, prefill_splits(prefill_tiles(n, 1, G), n_kv, long_row, head_dim), head_dim);
         most = b > most ? b : most;
     }
-    return most;
+    const int64_t four = max_reqs > 0 ? kv4_workspace(max_reqs, n_kv, G, head_dim) : 0;
+    return four > most ? four : most;
 }
 
 extern "C" int32_t locks_window_decode(
