@@ -44,6 +44,29 @@ int launch_decode_range(const uint16_t* q, long q_sr, long q_sh, const uint16_t*
                         int head_dim, int page, float scale, hipStream_t stream);
 
 constexpr int AT_MAX_SPLITS = 128;          // of one row, all kinds together
+constexpr int AT_ROWS = 128;                // query rows (token, head of the group) of a prompt's workgroup
+constexpr float kLog2e = 1.44269504088896340736f;
+
+typedef float v16f __attribute__((ext_vector_type(16)));
+typedef short v4s __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) v4s* lds_v4s;
+
+__device__ __forceinline__ int wave_max_int(int v) { return (int)(wave_max_u32((uint32_t)v ^ 0x80000000u) ^ 0x80000000u); }
+__device__ __forceinline__ int wave_min_int(int v) { return ~wave_max_int(~v); }
+
+inline int clampi(long x, int lo, int hi) { return (int)(x < lo ? lo : x > hi ? hi : x); }
+// Tiles of k non-empty requests (groups) of n tokens together: sum of ceil(c / TQ)
+// <= floor((n - k) / TQ) + k, largest where all are non-empty.
+inline long prefill_tiles(int n_tokens, int n_req, int G) {
+    const int k = n_req < n_tokens ? n_req : n_tokens;
+    return (long)(n_tokens - k) / (AT_ROWS / G) + k;
+}
+// The keys that a host-side bound leaves.
+inline long bound_keys(int32_t max_seq_len, int32_t bt_cols, int32_t page) {
+    const long cap = (long)bt_cols * page;
+    return max_seq_len > 0 && max_seq_len < cap ? max_seq_len : cap;
+}
+
 
 // Joins the partials of every row (locks_window.hip); with `starts` only of the rows
 // of starts[0] .. starts[n_seq].
@@ -70,5 +93,7 @@ int32_t check_kv4(const char* what, const void* cache, int64_t sb, int64_t sh, i
 
 // Workspace of a single-token call on one (locks_kv4.hip).
 int64_t kv4_workspace(int n_req, int n_kv, int G, int head_dim);
+// Splits of a row's keys in a call of many tokens on one.
+int kv4_prefill_splits(long tiles, int n_kv, long max_keys, int head_dim);
 
 }  // namespace locks

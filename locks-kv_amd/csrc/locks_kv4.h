@@ -60,31 +60,41 @@ struct Kv4Lane {
     uint32_t w[D / 32];
     uint32_t s;                                     // K: one or two scale bytes; V: one of each token
 };
-template <int D>
-__device__ __forceinline__ void kv4_codes(const uint8_t* p, int lane, uint32_t* w) {
+// (by pointers of the global address space: an address put together from integers would
+// be loaded from through the path that LDS shares)
+typedef const __attribute__((address_space(1))) uint8_t* kv4_ptr;
+// NT: read once (decode), so past the caches; a prompt's tiles are read by all its rows.
+template <typename T, bool NT>
+__device__ __forceinline__ T kv4_read(kv4_ptr p) {
+    const __attribute__((address_space(1))) T* q = (const __attribute__((address_space(1))) T*)p;
+    if constexpr (NT) return __builtin_nontemporal_load(q);
+    else return *q;
+}
+template <int D, bool NT>
+__device__ __forceinline__ void kv4_codes(kv4_ptr p, int lane, uint32_t* w) {
     if constexpr (D == 64) {
-        const v2i x = __builtin_nontemporal_load(reinterpret_cast<const v2i*>(p + lane * 8));
+        const v2i x = kv4_read<v2i, NT>(p + lane * 8);
         w[0] = x[0]; w[1] = x[1];
     } else {
 #pragma unroll
         for (int i = 0; i < D / 128; ++i) {
-            const v4i x = __builtin_nontemporal_load(reinterpret_cast<const v4i*>(p + i * 1024 + lane * 16));
+            const v4i x = kv4_read<v4i, NT>(p + i * 1024 + lane * 16);
             w[4 * i] = x[0]; w[4 * i + 1] = x[1]; w[4 * i + 2] = x[2]; w[4 * i + 3] = x[3];
         }
     }
 }
-template <int D>
-__device__ __forceinline__ void kv4_load_k(const uint8_t* tile, int lane, Kv4Lane<D>& x) {
-    kv4_codes<D>(tile, lane, x.w);
+template <int D, bool NT>
+__device__ __forceinline__ void kv4_load_k(kv4_ptr tile, int lane, Kv4Lane<D>& x) {
+    kv4_codes<D, NT>(tile, lane, x.w);
     if constexpr (D == 64) x.s = tile[Kv4<D>::KS + (lane >> 5) * 16 + (lane & 15)];
     else if constexpr (D == 128) x.s = tile[Kv4<D>::KS + lane];
-    else x.s = *reinterpret_cast<const uint16_t*>(tile + Kv4<D>::KS + 2 * lane);
+    else x.s = *(const __attribute__((address_space(1))) uint16_t*)(tile + Kv4<D>::KS + 2 * lane);
 }
-template <int D>
-__device__ __forceinline__ void kv4_load_v(const uint8_t* tile, int lane, Kv4Lane<D>& x) {
-    kv4_codes<D>(tile + Kv4<D>::VC, lane, x.w);
+template <int D, bool NT>
+__device__ __forceinline__ void kv4_load_v(kv4_ptr tile, int lane, Kv4Lane<D>& x) {
+    kv4_codes<D, NT>(tile + Kv4<D>::VC, lane, x.w);
     const int blk = (lane & 15) * (D / 16) / 32;
-    x.s = *reinterpret_cast<const uint32_t*>(tile + Kv4<D>::VS + ((lane >> 4) * Kv4<D>::NBLK + blk) * 4);
+    x.s = *(const __attribute__((address_space(1))) uint32_t*)(tile + Kv4<D>::VS + ((lane >> 4) * Kv4<D>::NBLK + blk) * 4);
 }
 
 // The scale 2^e of a byte as the converters take it (255: infinite, whose entries

@@ -34,7 +34,7 @@ constexpr int K4_BLK = K4_WAVES * kWave;
 constexpr int K4_TILES = 2;                 // of a wave's step
 constexpr int K4_ROW = 32;                  // a row's start (query, first loads, output) in tiles' time
 constexpr int K4_SHARE = 24;                // tiles that a share has at least
-constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
+constexpr float kLn2 = 0.69314718055994530942f;
 
 struct Kv4DecodeArgs {
     const uint16_t* q; long q_sr, q_sh;
@@ -221,11 +221,11 @@ __global__ __launch_bounds__(K4_BLK, 2) void kv4_decode_kernel(const Kv4DecodeAr
         x.edge = (edges >> l0 & ((1u << T) - 1)) != 0;
 #pragma unroll
         for (int t = 0; t < T; ++t) {
-            const uint8_t* p = reinterpret_cast<const uint8_t*>((uint64_t)(uint32_t)__builtin_amdgcn_readlane(at_lo, l0 + t) |
-                                                                (uint64_t)(uint32_t)__builtin_amdgcn_readlane(at_hi, l0 + t) << 32);
+            const kv4_ptr p = (kv4_ptr)((uint64_t)(uint32_t)__builtin_amdgcn_readlane(at_lo, l0 + t) |
+                                        (uint64_t)(uint32_t)__builtin_amdgcn_readlane(at_hi, l0 + t) << 32);
             x.key0[t] = __builtin_amdgcn_readlane(key_of, l0 + t);
-            kv4_load_k<D>(p, lane, x.k[t]);
-            kv4_load_v<D>(p, lane, x.v[t]);
+            kv4_load_k<D, true>(p, lane, x.k[t]);
+            kv4_load_v<D, true>(p, lane, x.v[t]);
         }
     };
 
@@ -551,8 +551,7 @@ extern "C" int32_t locks_kv4_decode(
                     out_stride_head, n_req, n_kv, G, head_dim, page, max_seq_len, scale);
     if (rc) return rc;
     if (n_req == 0) return 0;
-    long keys = (long)bt_cols * page;
-    if (max_seq_len > 0 && max_seq_len < keys) keys = max_seq_len;
+    long keys = bound_keys(max_seq_len, bt_cols, page);
     if (window && (long)window + sinks + 32 < keys) keys = (long)window + sinks + 32;
     Kv4DecodeArgs a{q, q_stride_req, q_stride_head, cache, c_stride_block, c_stride_head, block_table, bt_stride, seq_lens,
                     out, out_stride_req, out_stride_head, lse, lse_stride_req, nullptr, nullptr, nullptr, nullptr,

@@ -34,7 +34,6 @@
 #include "locks_attn.h"
 #include "locks_common.h"
 #include "locks_hip.h"
-#include "locks_kv4.h"
 
 #include <math.h>
 
@@ -43,15 +42,10 @@
 namespace locks {
 
 typedef __attribute__((address_space(3))) void* lds_ptr;
-typedef short v4s __attribute__((ext_vector_type(4)));
-typedef __attribute__((address_space(3))) v4s* lds_v4s;
-typedef float v16f __attribute__((ext_vector_type(16)));
 typedef unsigned short v2us __attribute__((ext_vector_type(2)));
 
 constexpr int AT_WAVES = 4;
 constexpr int AT_BLK = AT_WAVES * kWave;
-constexpr int AT_ROWS = 32 * AT_WAVES;      // query rows per workgroup
-constexpr float kLog2e = 1.44269504088896340736f;
 
 template <int D>
 struct AtGeom {
@@ -65,6 +59,8 @@ struct AtGeom {
     static __device__ __forceinline__ int swz_k(int row) { return D == 64 ? (row >> 1) & 7 : row & 15; }
     static __device__ __forceinline__ int swz_v(int row) { return D == 64 ? ((row >> 1) & 1) << 2 : (row & 3) << 2; }
 };
+
+static_assert(AT_ROWS == 32 * AT_WAVES, "query rows per workgroup");
 
 constexpr int vm_wait(int n) { return 0x0F70 | (n & 15) | ((n >> 4) << 14); }    // s_waitcnt vmcnt(n)
 
@@ -84,15 +80,12 @@ struct TileArgs {
     int NB, bt_cols, n_rows, n_seq, n_kv, G, pg_sh, window, sinks, nsplit;
     int own;                                // SHARED: splits of a request's own keys, behind the nsplit of its prefix
     int shared_units, own_units, chunk;     // and how the two kinds of work are dealt out (per kv head)
-    const uint8_t* c4; long c_sb, c_sh;     // KV4: the cache, in place of k and v
 };
 
 // 16 bytes per lane from its own address to 1 KB of LDS, in lane order
 __device__ __forceinline__ void load_lds16(const uint8_t* src, uint8_t* dst) {
     __builtin_amdgcn_global_load_lds(src, (lds_ptr)dst, 16, 0, 0);
 }
-__device__ __forceinline__ int wave_max_int(int v) { return (int)(wave_max_u32((uint32_t)v ^ 0x80000000u) ^ 0x80000000u); }
-__device__ __forceinline__ int wave_min_int(int v) { return ~wave_max_int(~v); }
 // bit 0 / 1: the low / high bf16 of a word is infinite or NaN
 __device__ __forceinline__ uint32_t nonfinite2(uint32_t w) {
     return ((w & 0x7F80u) == 0x7F80u ? 1u : 0u) | ((w & 0x7F800000u) == 0x7F800000u ? 2u : 0u);
@@ -103,20 +96,16 @@ __device__ __forceinline__ uint32_t nonfinite2(uint32_t w) {
 // partials only.  The prefix is bound by the matrix cores, own keys by memory: dealt
 // out in turns of one workgroup per CU, they overlap.
 // PART: partials instead of the output.
-// KV4: the cache holds 4 bits an entry.  A wave loads its share of a tile as codes, a
-// tile ahead of the one it converts, and writes the converted rows to the same places
-// in LDS: a tile is converted once for its 128 query rows.
-template <int D, bool SHARED, bool PART, bool KV4>
+template <int D, bool SHARED, bool PART>
 __global__ __launch_bounds__(AT_BLK, D == 256 ? 1 : 2) void attn_tile_kernel(const TileArgs a)
 {
     using GM = AtGeom<D>;
     constexpr int KT = GM::KT, ROWB = GM::ROWB, NB2 = KT / 32, ND = D / 32;
     constexpr int VPRE = D == 256 ? ND / 2 : ND;        // column blocks of V read before the softmax
     static_assert(!SHARED || PART, "a prefix is one part of a row");
-    static_assert(!SHARED || !KV4, "a prefix is in bf16");
     // one array per tile: the compiler can tell the DMA of one from the reads of
     // another, and waits for neither
-    constexpr int NST = KV4 ? 2 : GM::NST, TB = GM::TILEB;
+    constexpr int NST = GM::NST, TB = GM::TILEB;
     __shared__ __attribute__((aligned(1024))) uint8_t k0[TB], k1[TB], k2[NST > 2 ? TB : 16];
     __shared__ __attribute__((aligned(1024))) uint8_t v0[TB], v1[TB], v2[NST > 2 ? TB : 16];
     static_assert(NST == 2 || NST == 3, "tiles in LDS");
@@ -279,7 +268,7 @@ __global__ __launch_bounds__(AT_BLK, D == 256 ? 1 : 2) void attn_tile_kernel(con
     // byte offsets of this lane's 16-byte chunks from the wave's first row
     uint32_t ko[GM::NI], vo[GM::NI];
 #pragma unroll
-    for (int i = 0; i < GM::NI && !KV4; ++i) {
+    for (int i = 0; i < GM::NI; ++i) {
         const int at = i * 1024 + lane * 16, row = at / ROWB, slot = (at % ROWB) / 16;
         const int tr = wave * GM::WROWS + row;              // row of the tile
         ko[i] = (uint32_t)(row * a.k_st * 2) + 16 * (slot ^ GM::swz_k(tr));
@@ -295,49 +284,6 @@ __global__ __launch_bounds__(AT_BLK, D == 256 ? 1 : 2) void attn_tile_kernel(con
         for (int i = 0; i < GM::NI; ++i) {
             load_lds16(kp + ko[i], kb + wave * GM::WROWS * ROWB + i * 1024);
             load_lds16(vp + vo[i], vb + wave * GM::WROWS * ROWB + i * 1024);
-        }
-    };
-
-    // KV4: this wave's codes of a tile: 16 rows of K and V, or at d 256, where a tile
-    // has 32 rows, K (even waves) or V of them
-    constexpr bool BOTH = KT == 64;
-    Kv4Lane<D> ck, cv;
-    auto load_codes = [&](int n) __attribute__((always_inline)) {
-        if (n - ids0 >= kWave) fetch_ids(n);
-        const long blk = __builtin_amdgcn_readlane(ids, n - ids0);
-        const int off = (key_of(n) + wave * GM::WROWS) & ((1 << a.pg_sh) - 1);
-        const uint8_t* p = a.c4 + blk * a.c_sb + (long)kh * a.c_sh + (off >> 4) * Kv4<D>::TILE;
-        if (BOTH || !(wave & 1)) kv4_load_k<D>(p, lane, ck);
-        if (BOTH || (wave & 1)) kv4_load_v<D>(p, lane, cv);
-    };
-    auto write_rows = [&](uint8_t* kb, uint8_t* vb) __attribute__((always_inline)) {
-        const int row0 = 16 * (BOTH ? wave : wave >> 1), r16 = lane & 15, kg = lane >> 4;
-        auto put = [&](uint8_t* buf, int row, int chunk, int swz, const uint4& x) __attribute__((always_inline)) {
-            *reinterpret_cast<uint4*>(buf + row * ROWB + ((chunk ^ swz) * 16)) = x;
-        };
-        if (BOTH || !(wave & 1)) {                      // lane: entries kg D / 4 .. of one token
-            const int row = row0 + r16;
-#pragma unroll
-            for (int st = 0; st < D / 32; ++st)
-                put(kb, row, kg * (D / 32) + st, GM::swz_k(row),
-                    kv4_eight(ck.w[st], kv4_scale(ck.s, D == 256 ? st >> 2 : 0)));
-        }
-        if (BOTH || (wave & 1)) {                       // lane: entries r16 D / 16 .. of four tokens
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int row = row0 + 4 * kg + i;
-                const float sc = kv4_scale(cv.s, i);
-                if constexpr (D == 64) {
-                    const uint32_t w = cv.w[i >> 1];
-                    const uint2 x = (i & 1) ? make_uint2(kv4_pair<2>(w, sc), kv4_pair<3>(w, sc))
-                                            : make_uint2(kv4_pair<0>(w, sc), kv4_pair<1>(w, sc));
-                    *reinterpret_cast<uint2*>(vb + row * ROWB + (((r16 >> 1) ^ GM::swz_v(row)) * 16) + (r16 & 1) * 8) = x;
-                } else {
-#pragma unroll
-                    for (int j = 0; j < D / 128; ++j)
-                        put(vb, row, r16 * (D / 128) + j, GM::swz_v(row), kv4_eight(cv.w[i * (D / 128) + j], sc));
-                }
-            }
         }
     };
 
@@ -526,17 +472,6 @@ __global__ __launch_bounds__(AT_BLK, D == 256 ? 1 : 2) void attn_tile_kernel(con
     // Tile n is in LDS once at most the loads of the tiles behind it are under way,
     // and free for the next one once every wave has passed the barrier after it.
     auto tile_step = [&](int n, auto use, auto fill) __attribute__((always_inline)) {
-        if constexpr (KV4) {
-            // every wave has written its rows of tile n and is through with the tile
-            // before it, whose place the codes on hand take
-            lds_barrier();
-            if (n + 1 < n1) {
-                write_rows(kbuf(fill), vbuf(fill));
-                if (n + 2 < n1) load_codes(n + 2);
-            }
-            compute(n, kbuf(use), vbuf(use));
-            return;
-        }
         const int behind = min(n1 - 1 - n, NST - 2);
         if (behind == 0) __builtin_amdgcn_s_waitcnt(vm_wait(0));
         else __builtin_amdgcn_s_waitcnt(vm_wait(2 * GM::NI));
@@ -548,13 +483,7 @@ __global__ __launch_bounds__(AT_BLK, D == 256 ? 1 : 2) void attn_tile_kernel(con
     using I2 = std::integral_constant<int, 2>;
     if (n0 < n1) {
         fetch_ids(n0);
-        if constexpr (KV4) {
-            load_codes(n0);
-            write_rows(k0, v0);
-            if (n0 + 1 < n1) load_codes(n0 + 1);
-        } else {
-            stage(n0, k0, v0);
-        }
+        stage(n0, k0, v0);
         if constexpr (NST > 2) { if (n0 + 1 < n1) stage(n0 + 1, k1, v1); }
     }
     for (int n = n0; n < n1; n += NST) {
@@ -685,7 +614,6 @@ __global__ __launch_bounds__(AM_BLK) void attn_merge_kernel(const Partials p, ui
 }
 
 // ---- launch shapes: host integers only, so that a captured call keeps them ----
-static int clampi(long x, int lo, int hi) { return (int)(x < lo ? lo : x > hi ? hi : x); }
 
 // A single-token call: about 512 workgroups (two per CU), each of at least 8
 // 16-token steps (two per wave).  With `even`, a row's splits hold at most 64 steps:
@@ -698,12 +626,6 @@ static int decode_splits(int n_req, int n_kv, long max_keys, bool even) {
     const long fill = (512 + rows - 1) / rows, cap = (4096 + rows - 1) / rows;
     const long most = !even ? 1 : (steps + 63) / 64 < cap ? (steps + 63) / 64 : cap;
     return clampi(fill > most ? fill : most, 1, clampi((steps + 7) / 8, 1, 64));
-}
-// Tiles of k non-empty requests (groups) of n tokens together: sum of ceil(c / TQ)
-// <= floor((n - k) / TQ) + k, largest where all are non-empty.
-static long prefill_tiles(int n_tokens, int n_req, int G) {
-    const int k = n_req < n_tokens ? n_req : n_tokens;
-    return (long)(n_tokens - k) / (AT_ROWS / G) + k;
 }
 // Many tokens: one split once there are 256 workgroups, else about 512 of at
 // least 4 key tiles.
@@ -767,11 +689,6 @@ int32_t check_ws(const char* what, const void* ws, int64_t have, int64_t need)
 
 using namespace locks;
 
-static long bound_keys(int32_t max_seq_len, int32_t bt_cols, int32_t page) {
-    const long cap = (long)bt_cols * page;
-    return max_seq_len > 0 && max_seq_len < cap ? max_seq_len : cap;
-}
-
 extern "C" int64_t locks_attn_workspace_bytes(int32_t max_reqs, int32_t max_tokens, int32_t n_kv, int32_t G,
                                               int32_t head_dim)
 {
@@ -792,8 +709,16 @@ extern "C" int64_t locks_attn_workspace_bytes(int32_t max_reqs, int32_t max_toke
         const int64_t b = part_bytes((int64_t)n * n_kv * G, prefill_splits(prefill_tiles(n, 1, G), n_kv, long_row, head_dim), head_dim);
         most = b > most ? b : most;
     }
-    const int64_t four = max_reqs > 0 ? kv4_workspace(max_reqs, n_kv, G, head_dim) : 0;
-    return four > most ? four : most;
+    // the same calls on a cache in 4 bits
+    if (max_reqs > 0) {
+        const int64_t b = kv4_workspace(max_reqs < 65535 ? max_reqs : 65535, n_kv, G, head_dim);
+        most = b > most ? b : most;
+    }
+    for (int n = 1; n <= max_tokens && prefill_tiles(n, 1, G) * n_kv < 256; ++n) {
+        const int64_t b = part_bytes((int64_t)n * n_kv * G, kv4_prefill_splits(prefill_tiles(n, 1, G), n_kv, long_row, head_dim), head_dim);
+        most = b > most ? b : most;
+    }
+    return most;
 }
 
 extern "C" int32_t locks_window_decode(
@@ -827,47 +752,12 @@ extern "C" int32_t locks_window_decode(
     return launch_merge(p, out, out_stride_req, out_stride_head, lse, lse_stride_req, n_req, n_kv, G, head_dim, nullptr, 0, st);
 }
 
-#define AT_LAUNCH_D(D, SHARED, PART, KV4) \
-    hipLaunchKernelGGL((attn_tile_kernel<D, SHARED, PART, KV4>), grid, dim3(AT_BLK), 0, st, a)
-#define AT_LAUNCH(SHARED, PART, KV4)                                    \
-    do {                                                                \
-        if (head_dim == 64) AT_LAUNCH_D(64, SHARED, PART, KV4);         \
-        else if (head_dim == 128) AT_LAUNCH_D(128, SHARED, PART, KV4);  \
-        else AT_LAUNCH_D(256, SHARED, PART, KV4);                       \
+#define AT_LAUNCH(SHARED, PART)                                                                                     \
+    do {                                                                                                            \
+        if (head_dim == 64) hipLaunchKernelGGL((attn_tile_kernel<64, SHARED, PART>), grid, dim3(AT_BLK), 0, st, a);  \
+        else if (head_dim == 128) hipLaunchKernelGGL((attn_tile_kernel<128, SHARED, PART>), grid, dim3(AT_BLK), 0, st, a); \
+        else hipLaunchKernelGGL((attn_tile_kernel<256, SHARED, PART>), grid, dim3(AT_BLK), 0, st, a);                \
     } while (0)
-
-// A call of many tokens, on the cache that `a` names; `a` without its partials and
-// launch shape.
-static int32_t prefill(const char* what, TileArgs a, const int32_t* query_start_loc, void* workspace,
-                       int64_t workspace_bytes, int32_t head_dim, int32_t page, int32_t max_seq_len, bool kv4, hipStream_t st)
-{
-    LOCKS_REQUIRE(query_start_loc, "%s: null pointer argument", what);
-    LOCKS_REQUIRE(a.n_rows >= 0, "%s: n_tokens %d < 0", what, a.n_rows);
-    if (a.n_seq == 0 || a.n_rows == 0) return 0;
-    const long bound = bound_keys(max_seq_len, a.bt_cols, page), reach = (long)a.window + a.sinks + a.n_rows;
-    const long tiles = prefill_tiles(a.n_rows, a.n_seq, a.G);
-    const int ns = prefill_splits(tiles, a.n_kv, a.window && reach < bound ? reach : bound, head_dim);
-    const int64_t rows = (int64_t)a.n_rows * a.n_kv * a.G;
-    LOCKS_REQUIRE(tiles * a.n_kv * ns <= 0x7fffffffL, "%s: too many tokens and heads for one launch", what);
-    if (ns > 1) {
-        const int rc = check_ws(what, workspace, workspace_bytes, part_bytes(rows, ns, head_dim));
-        if (rc) return rc;
-        a.p = part_layout(workspace, rows, ns, head_dim);
-    }
-    a.nsplit = ns;
-    const dim3 grid((unsigned)(tiles * a.n_kv * ns));
-    if (ns == 1) {
-        if (kv4) AT_LAUNCH(false, false, true);
-        else AT_LAUNCH(false, false, false);
-        return check_launch("attn_tile_kernel");
-    }
-    if (kv4) AT_LAUNCH(false, true, true);
-    else AT_LAUNCH(false, true, false);
-    const int rc = check_launch("attn_tile_kernel<part>");
-    if (rc) return rc;
-    return launch_merge(a.p, a.out, a.o_st, a.o_sh, a.lse, a.lse_st, a.n_rows, a.n_kv, a.G, head_dim, query_start_loc,
-                        a.n_seq, st);
-}
 
 extern "C" int32_t locks_window_prefill(
     const uint16_t* q, int64_t q_stride_tok, int64_t q_stride_head, const uint16_t* k_cache, int64_t k_stride_block,
@@ -880,40 +770,36 @@ extern "C" int32_t locks_window_prefill(
 {
     const char* what = "locks_window_prefill";
     const int64_t ks64[3] = {k_stride_block, k_stride_tok, k_stride_head}, vs64[3] = {v_stride_block, v_stride_tok, v_stride_head};
-    const int rc = check_attn(what, q, q_stride_tok, q_stride_head, k_cache, ks64, v_cache, vs64, num_blocks, block_table,
-                              bt_stride, bt_cols, seq_lens, window, sinks, out, out_stride_tok, out_stride_head, n_req, n_kv,
-                              G, head_dim, page, max_seq_len, scale);
+    int rc = check_attn(what, q, q_stride_tok, q_stride_head, k_cache, ks64, v_cache, vs64, num_blocks, block_table, bt_stride,
+                        bt_cols, seq_lens, window, sinks, out, out_stride_tok, out_stride_head, n_req, n_kv, G, head_dim,
+                        page, max_seq_len, scale);
     if (rc) return rc;
+    LOCKS_REQUIRE(query_start_loc, "%s: null pointer argument", what);
+    LOCKS_REQUIRE(n_tokens >= 0, "%s: n_tokens %d < 0", what, n_tokens);
+    if (n_req == 0 || n_tokens == 0) return 0;
+    const long keys = window ? (long)window + sinks + n_tokens : bound_keys(max_seq_len, bt_cols, page);
+    const long tiles = prefill_tiles(n_tokens, n_req, G);
+    int ns = prefill_splits(tiles, n_kv, keys < bound_keys(max_seq_len, bt_cols, page) ? keys : bound_keys(max_seq_len, bt_cols, page), head_dim);
+    const int64_t rows = (int64_t)n_tokens * n_kv * G;
+    LOCKS_REQUIRE(tiles * n_kv * ns <= 0x7fffffffL, "%s: too many tokens and heads for one launch", what);
+    Partials p{};
+    if (ns > 1) {
+        rc = check_ws(what, workspace, workspace_bytes, part_bytes(rows, ns, head_dim));
+        if (rc) return rc;
+        p = part_layout(workspace, rows, ns, head_dim);
+    }
     const TileArgs a{q, q_stride_tok, q_stride_head, k_cache, k_stride_block, k_stride_tok, k_stride_head, v_cache,
                      v_stride_block, v_stride_tok, v_stride_head, block_table, bt_stride, seq_lens, query_start_loc, nullptr,
-                     out, out_stride_tok, out_stride_head, lse, lse_stride_tok, Partials{}, scale * kLog2e, scale, num_blocks,
-                     bt_cols, n_tokens, n_req, n_kv, G, page == 16 ? 4 : page == 32 ? 5 : 6, window, sinks, 1, 0, 0, 0, 1,
-                     nullptr, 0, 0};
-    return prefill(what, a, query_start_loc, workspace, workspace_bytes, head_dim, page, max_seq_len, false, (hipStream_t)stream);
-}
-
-extern "C" int32_t locks_kv4_prefill(
-    const uint16_t* q, int64_t q_stride_tok, int64_t q_stride_head, const uint8_t* cache, int64_t c_stride_block,
-    int64_t c_stride_head, int32_t num_blocks, const int32_t* block_table, int64_t bt_stride, int32_t bt_cols,
-    const int32_t* seq_lens, const int32_t* query_start_loc, int32_t window, int32_t sinks, uint16_t* out,
-    int64_t out_stride_tok, int64_t out_stride_head, float* lse, int64_t lse_stride_tok, void* workspace,
-    int64_t workspace_bytes, int32_t n_tokens, int32_t n_req, int32_t n_kv, int32_t G, int32_t head_dim, int32_t page,
-    int32_t max_seq_len, float scale, void* stream)
-{
-    const char* what = "locks_kv4_prefill";
-    int rc = check_kv4(what, cache, c_stride_block, c_stride_head, num_blocks, n_kv, head_dim, page);
+                     out, out_stride_tok, out_stride_head, lse, lse_stride_tok, p, scale * kLog2e, scale, num_blocks, bt_cols,
+                     n_tokens, n_req, n_kv, G, page == 16 ? 4 : page == 32 ? 5 : 6, window, sinks, ns, 0, 0, 0, 1};
+    hipStream_t st = (hipStream_t)stream;
+    const dim3 grid((unsigned)(tiles * n_kv * ns));
+    if (ns == 1) { AT_LAUNCH(false, false); return check_launch("attn_tile_kernel"); }
+    AT_LAUNCH(false, true);
+    rc = check_launch("attn_tile_kernel<part>");
     if (rc) return rc;
-    const int64_t none[3] = {0, 0, 0};
-    const uint16_t* any = reinterpret_cast<const uint16_t*>(cache);
-    rc = check_attn(what, q, q_stride_tok, q_stride_head, any, none, any, none, num_blocks, block_table, bt_stride, bt_cols,
-                    seq_lens, window, sinks, out, out_stride_tok, out_stride_head, n_req, n_kv, G, head_dim, page,
-                    max_seq_len, scale);
-    if (rc) return rc;
-    const TileArgs a{q, q_stride_tok, q_stride_head, nullptr, 0, 0, 0, nullptr, 0, 0, 0, block_table, bt_stride, seq_lens,
-                     query_start_loc, nullptr, out, out_stride_tok, out_stride_head, lse, lse_stride_tok, Partials{},
-                     scale * kLog2e, scale, num_blocks, bt_cols, n_tokens, n_req, n_kv, G,
-                     page == 16 ? 4 : page == 32 ? 5 : 6, window, sinks, 1, 0, 0, 0, 1, cache, c_stride_block, c_stride_head};
-    return prefill(what, a, query_start_loc, workspace, workspace_bytes, head_dim, page, max_seq_len, true, (hipStream_t)stream);
+    return launch_merge(p, out, out_stride_tok, out_stride_head, lse, lse_stride_tok, n_tokens, n_kv, G, head_dim,
+                        query_start_loc, n_req, st);
 }
 
 extern "C" int32_t locks_prefix_decode(
@@ -948,10 +834,10 @@ extern "C" int32_t locks_prefix_decode(
                      v_stride_block, v_stride_tok, v_stride_head, block_table, bt_stride, seq_lens, group_start, prefix_pages,
                      nullptr, 0, 0, nullptr, 0, p, scale * kLog2e, scale, num_blocks, bt_cols, n_req, n_groups, n_kv, G,
                      page == 16 ? 4 : page == 32 ? 5 : 6, 0, 0, shr, own, (int)(tiles * shr), n_req * own,
-                     n_kv < 256 ? 256 / n_kv : 1, nullptr, 0, 0};
+                     n_kv < 256 ? 256 / n_kv : 1};
     hipStream_t st = (hipStream_t)stream;
     const dim3 grid((unsigned)((tiles * shr + (long)n_req * own) * n_kv));
-    AT_LAUNCH(true, true, false);
+    AT_LAUNCH(true, true);
     rc = check_launch("attn_tile_kernel<shared>");
     if (rc) return rc;
     return launch_merge(p, out, out_stride_req, out_stride_head, lse, lse_stride_req, n_req, n_kv, G, head_dim, nullptr, 0, st);

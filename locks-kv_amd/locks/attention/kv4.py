@@ -43,8 +43,32 @@ def kv4_read(kv_cache, slots, k_out, v_out) -> None:
     """Rows ``slots`` (T,) int64 (block * page + offset) of a cache in 4 bits as bf16
     (T, n_kv, d): the values that the codes stand for, exactly.  A slot outside the
     cache (padding: -1) leaves its rows as they were."""
-    _, page, n_kv, d = kv4_geometry("kv4_read", kv_cache)
+    # one pass over the tensors' attributes (as qk_norm_rope_write); _refuse_read has the messages
     index = kv_cache.get_device()
+    try:
+        (NB, n_kv, tiles, rec), (cb, ch, ct, c1) = kv_cache.shape, kv_cache.stride()
+        (n,), (ss,) = slots.shape, slots.stride()
+        (tk, hk, dk), (tv, hv, dv) = k_out.shape, v_out.shape
+        (k0, k1, k2), (v0, v1, v2) = k_out.stride(), v_out.stride()
+        d = rec // 17
+        ok = (index >= 0 and kv_cache.dtype is _U8 and rec % 17 == 0 and ct == rec and c1 == 1 and slots.dtype is _I64
+              and (ss == 1 or n < 2) and k_out.dtype is _BF16 and v_out.dtype is _BF16 and k2 == 1 and v2 == 1
+              and tk >= n and tv >= n and hk == n_kv and hv == n_kv and dk == d and dv == d
+              and slots.get_device() == index and k_out.get_device() == index and v_out.get_device() == index)
+    except ValueError:                                       # another number of dims
+        ok = False
+    if not ok:
+        _refuse_read(kv_cache, slots, k_out, v_out)
+    if n == 0:
+        return
+    _lib.launch("locks_kv4_read", index, (
+        kv_cache.data_ptr(), cb, ch, NB, slots.data_ptr(), k_out.data_ptr(), k0, k1, v_out.data_ptr(), v0, v1, n, n_kv, d,
+        16 * tiles))
+
+
+def _refuse_read(kv_cache, slots, k_out, v_out) -> None:
+    """The error of a call that kv4_read does not take."""
+    _, _, n_kv, d = kv4_geometry("kv4_read", kv_cache)
     if slots.dtype is not _I64 or slots.dim() != 1 or not slots.is_contiguous():
         raise TypeError(f"kv4_read: slots must be a contiguous int64 vector, got {slots.dtype} {tuple(slots.shape)}")
     n = slots.shape[0]
@@ -54,12 +78,5 @@ def kv4_read(kv_cache, slots, k_out, v_out) -> None:
                             f"{tuple(t.shape)} strides {t.stride()}")
         if t.shape[0] < n or t.shape[1] != n_kv or t.shape[2] != d:
             raise ValueError(f"kv4_read: {name} has shape {tuple(t.shape)}, the call needs ({n}, {n_kv}, {d})")
-    if index < 0 or any(t.get_device() != index for t in (slots, k_out, v_out)):
-        raise ValueError(f"kv4_read runs on one GPU: the cache is on {kv_cache.device}, slots on {slots.device}, outputs on "
-                         f"{k_out.device} and {v_out.device}")
-    if n == 0:
-        return
-    _lib.launch("locks_kv4_read", index, (
-        kv_cache.data_ptr(), kv_cache.stride(0), kv_cache.stride(1), kv_cache.shape[0], slots.data_ptr(),
-        k_out.data_ptr(), k_out.stride(0), k_out.stride(1), v_out.data_ptr(), v_out.stride(0), v_out.stride(1), n, n_kv,
-        d, page))
+    raise ValueError(f"kv4_read runs on one GPU: the cache is on {kv_cache.device}, slots on {slots.device}, outputs on "
+                     f"{k_out.device} and {v_out.device}")
