@@ -393,86 +393,86 @@ __global__ __launch_bounds__(K4_BLK, 2) void kv4_decode_kernel(const Kv4DecodeAr
     }
 }
 
-// Joins the shares of every row that has several: one workgroup per (request, head),
-// D / 4 columns of K4_BLK 4 / D streams over the shares.  The first share's partial is in
-// its second slot (it starts the row), the others' in their first.
+// Joins the shares of every row that has several: `hpw` heads of a row a workgroup (all
+// that fit where there are many rows, one where there are few), D / 4 columns each, and
+// what threads are left as streams over the shares.  The first share's partial is in its
+// second slot (it starts the row), the others' in their first.
 constexpr int K4_GRID = 512;                // shares at most: two workgroups a CU
-template <int D>
-__global__ __launch_bounds__(K4_BLK) void kv4_merge_kernel(const Kv4DecodeArgs a)
+template <int D, bool ONE>
+__global__ __launch_bounds__(K4_BLK) void kv4_merge_kernel(const Kv4DecodeArgs a, int heads)
 {
-    constexpr int COLS = D / 4, STREAMS = K4_BLK / COLS, PF = 8;
-    __shared__ float w_s[K4_GRID];
-    __shared__ float4 part[STREAMS][COLS];
-    const int tid = threadIdx.x, lane = tid & 63;
-    const int col = tid % COLS, strm = tid / COLS;
-    const int H = a.n_kv * a.G, hd = blockIdx.x % H, kh = hd / a.G, g = hd % a.G;
-    const long r = blockIdx.x / H;
-    const int2 sh = a.shares[r * a.n_kv + kh];
+    const int hpw = ONE ? 1 : heads;
+    constexpr int COLS = D / 4, PF = 8;
+    __shared__ float4 acc_s[K4_BLK];
+    __shared__ float2 ml_s[K4_BLK];
+    const int tid = threadIdx.x, col = tid % COLS, n_heads = (a.G + hpw - 1) / hpw;
+    const int hh = tid / COLS % hpw, strm = tid / (COLS * hpw), streams = K4_BLK / (COLS * hpw);
+    const long row = blockIdx.x / n_heads;          // request, kv head
+    const int g = blockIdx.x % n_heads * hpw + hh;
+    const int2 sh = a.shares[row];
     const int n = sh.y - sh.x + 1;
     if (n <= 0) return;
-    auto at = [&](int i) __attribute__((always_inline)) { return (2L * (sh.x + i) + (i == 0)) * a.G + g; };
-    // every load that needs no other goes out first; each wave makes all weights
-    float4 pre[PF];
-#pragma unroll
-    for (int k = 0; k < PF; ++k)
-        pre[k] = *reinterpret_cast<const float4*>(a.acc + at(min(strm + k * STREAMS, n - 1)) * D + 4 * col);
-    constexpr int NK = K4_GRID / kWave;
-    float ms[NK], ls[NK], mm = -INFINITY;
-#pragma unroll
-    for (int k = 0; k < NK; ++k) {
-        if (k * kWave >= n) break;
-        const int i = lane + k * kWave;
-        ls[k] = i < n ? a.l[at(i)] : 0.f;
-        ms[k] = i < n ? a.m[at(i)] : -INFINITY;
-        if (ls[k] == 0.f) ms[k] = -INFINITY;
-        mm = fmaxf(mm, ms[k]);
-    }
-    mm = wave_max(mm);
-    float lt = 0.f;
-#pragma unroll
-    for (int k = 0; k < NK; ++k) {
-        if (k * kWave >= n) break;
-        const int i = lane + k * kWave;
-        const float w = ls[k] == 0.f ? 0.f : mm == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ms[k] - mm);
-        lt += ls[k] * w;
-        if (tid < kWave && i < n) w_s[i] = w;
-    }
-    lt = wave_sum(lt);
-    __syncthreads();
+    const bool mine = strm < streams && g < a.G;
+    // the running maximum, sum and columns over this stream's shares
+    float m = -INFINITY, l = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    auto add = [&](float w, const float4& x) __attribute__((always_inline)) {
-        if (w != 0.f) { acc.x += w * x.x; acc.y += w * x.y; acc.z += w * x.z; acc.w += w * x.w; }
-    };
-#pragma unroll
-    for (int k = 0; k < PF; ++k) {
-        const int i = strm + k * STREAMS;
-        if (i < n) add(w_s[i], pre[k]);
-    }
-    for (int i0 = strm + PF * STREAMS; i0 < n; i0 += PF * STREAMS) {
-#pragma unroll
-        for (int k = 0; k < PF; ++k)
-            pre[k] = *reinterpret_cast<const float4*>(a.acc + at(min(i0 + k * STREAMS, n - 1)) * D + 4 * col);
+    for (int i0 = strm; mine && i0 < n; i0 += PF * streams) {
+        float4 x[PF];
+        float mi[PF], li[PF];
 #pragma unroll
         for (int k = 0; k < PF; ++k) {
-            const int i = i0 + k * STREAMS;
-            if (i < n) add(w_s[i], pre[k]);
+            const int i = min(i0 + k * streams, n - 1);
+            const long at = (2L * (sh.x + i) + (i == 0)) * a.G + g;
+            mi[k] = a.m[at];
+            li[k] = i0 + k * streams < n ? a.l[at] : 0.f;
+            x[k] = *reinterpret_cast<const float4*>(a.acc + at * D + 4 * col);
         }
-    }
-    part[strm][col] = acc;
-    __syncthreads();
-    if (tid < COLS) {
+        float top = m;
 #pragma unroll
-        for (int k = 1; k < STREAMS; ++k) {
-            const float4 x = part[k][tid];
-            acc.x += x.x; acc.y += x.y; acc.z += x.z; acc.w += x.w;
-        }
-        const float inv = lt == 0.f ? 0.f : 1.f / lt;
-        uint2 w;
-        w.x = (uint32_t)f32_to_bf16(acc.x * inv) | (uint32_t)f32_to_bf16(acc.y * inv) << 16;
-        w.y = (uint32_t)f32_to_bf16(acc.z * inv) | (uint32_t)f32_to_bf16(acc.w * inv) << 16;
-        *reinterpret_cast<uint2*>(a.out + r * a.o_sr + (long)hd * a.o_sh + 4 * tid) = w;
-        if (a.lse && tid == 0) a.lse[r * a.lse_sr + hd] = lt == 0.f ? -INFINITY : mm * kLn2 + logf(lt);
+        for (int k = 0; k < PF; ++k) top = fmaxf(top, li[k] == 0.f ? -INFINITY : mi[k]);
+        // (a maximum of -inf: every weight so far is 0 or NaN, and stays what it is)
+        const float old = top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - top);
+        l *= old;
+        acc.x *= old; acc.y *= old; acc.z *= old; acc.w *= old;
+#pragma unroll
+        for (int k = 0; k < PF; ++k)
+            if (li[k] != 0.f) {                     // a share without keys has no columns
+                const float w = top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mi[k] - top);
+                l += li[k] * w;
+                acc.x += w * x[k].x; acc.y += w * x[k].y; acc.z += w * x[k].z; acc.w += w * x[k].w;
+            }
+        m = top;
     }
+    if (streams > 1) {
+        acc_s[tid] = acc;
+        if (col == 0) ml_s[tid / COLS] = make_float2(m, l);
+        __syncthreads();
+        if (strm > 0 || !mine) return;
+        float top = m;
+#pragma unroll
+        for (int k = 1; k < streams; ++k) top = fmaxf(top, ml_s[k * hpw + hh].x);
+        acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        l = 0.f;
+#pragma unroll
+        for (int k = 0; k < streams; ++k) {
+            const float2 ml = ml_s[k * hpw + hh];
+            const float4 x = acc_s[tid + k * COLS * hpw];
+            if (ml.y == 0.f) continue;
+            const float w = top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ml.x - top);
+            l += ml.y * w;
+            acc.x += w * x.x; acc.y += w * x.y; acc.z += w * x.z; acc.w += w * x.w;
+        }
+        m = top;
+    }
+    if (!mine) return;
+    const long r = row / a.n_kv;
+    const int hd = (int)(row % a.n_kv) * a.G + g;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    uint2 w;
+    w.x = (uint32_t)f32_to_bf16(acc.x * inv) | (uint32_t)f32_to_bf16(acc.y * inv) << 16;
+    w.y = (uint32_t)f32_to_bf16(acc.z * inv) | (uint32_t)f32_to_bf16(acc.w * inv) << 16;
+    *reinterpret_cast<uint2*>(a.out + r * a.o_sr + (long)hd * a.o_sh + 4 * col) = w;
+    if (a.lse && col == 0) a.lse[r * a.lse_sr + hd] = l == 0.f ? -INFINITY : m * kLn2 + logf(l);
 }
 
 // ---- rows read back -------------------------------------------------------------
@@ -485,30 +485,46 @@ struct Kv4ReadArgs {
     int n_kv, pg_sh;
 };
 
-template <int D>
+// RD_UNITS units of a thread: their loads are in flight together.
+template <int D, int RD_UNITS>
 __global__ __launch_bounds__(256) void kv4_read_kernel(const Kv4ReadArgs a)
 {
     using L = Kv4<D>;
     constexpr int LPH = D / 8;
-    const long u = (long)blockIdx.x * 256 + threadIdx.x;
-    if (u >= a.units) return;
-    const int l = (int)(u % LPH), kh = (int)(u / LPH % a.n_kv);
-    const long t = u / LPH / a.n_kv;
-    const long slot = a.slots[t];
-    if (slot < 0 || slot >= a.n_slots) return;
-    const long blk = slot >> a.pg_sh;
-    const int off = (int)(slot & ((1 << a.pg_sh) - 1)), key = off & 15;
-    const uint8_t* p = a.c + blk * a.c_sb + (long)kh * a.c_sh + (off >> 4) * L::TILE;
-    const uint32_t kw = *reinterpret_cast<const uint32_t*>(p + L::k_code(key, l));
-    uint32_t vw;
-    if constexpr (D == 64)
-        vw = *reinterpret_cast<const uint16_t*>(p + L::v_code(key, l)) |
-             (uint32_t)*reinterpret_cast<const uint16_t*>(p + L::v_code(key, l) + 8) << 16;
-    else
-        vw = *reinterpret_cast<const uint32_t*>(p + L::v_code(key, l));
-    const float ks = kv4_scale(p[L::k_scale(key, l >> 2)], 0), vs = kv4_scale(p[L::v_scale(key, l >> 2)], 0);
-    *reinterpret_cast<uint4*>(a.k + t * a.k_st + (long)kh * a.k_sh + 8 * l) = kv4_eight(kw, ks);
-    *reinterpret_cast<uint4*>(a.v + t * a.v_st + (long)kh * a.v_sh + 8 * l) = kv4_eight(vw, vs);
+    const long u0 = (long)blockIdx.x * (256 * RD_UNITS) + threadIdx.x;
+    long slot[RD_UNITS], t[RD_UNITS];
+    int kh[RD_UNITS];
+    const int l = threadIdx.x % LPH;
+#pragma unroll
+    for (int k = 0; k < RD_UNITS; ++k) {
+        const long u = u0 + 256 * k, row = (u < a.units ? u : 0) / LPH;
+        t[k] = row / a.n_kv;
+        kh[k] = (int)(row - t[k] * a.n_kv);
+        slot[k] = u < a.units ? a.slots[t[k]] : -1;
+    }
+    uint32_t kw[RD_UNITS], vw[RD_UNITS], ks[RD_UNITS], vs[RD_UNITS];
+#pragma unroll
+    for (int k = 0; k < RD_UNITS; ++k) {
+        const bool here = slot[k] >= 0 && slot[k] < a.n_slots;
+        const long s = here ? slot[k] : 0;
+        slot[k] = here ? s : -1;
+        const int off = (int)(s & ((1 << a.pg_sh) - 1)), key = off & 15;
+        const uint8_t* p = a.c + (s >> a.pg_sh) * a.c_sb + (long)kh[k] * a.c_sh + (off >> 4) * L::TILE;
+        kw[k] = *reinterpret_cast<const uint32_t*>(p + L::k_code(key, l));
+        if constexpr (D == 64)
+            vw[k] = *reinterpret_cast<const uint16_t*>(p + L::v_code(key, l)) |
+                    (uint32_t)*reinterpret_cast<const uint16_t*>(p + L::v_code(key, l) + 8) << 16;
+        else
+            vw[k] = *reinterpret_cast<const uint32_t*>(p + L::v_code(key, l));
+        ks[k] = p[L::k_scale(key, l >> 2)];
+        vs[k] = p[L::v_scale(key, l >> 2)];
+    }
+#pragma unroll
+    for (int k = 0; k < RD_UNITS; ++k)
+        if (slot[k] >= 0) {
+            *reinterpret_cast<uint4*>(a.k + t[k] * a.k_st + (long)kh[k] * a.k_sh + 8 * l) = kv4_eight(kw[k], kv4_scale(ks[k], 0));
+            *reinterpret_cast<uint4*>(a.v + t[k] * a.v_st + (long)kh[k] * a.v_sh + 8 * l) = kv4_eight(vw[k], kv4_scale(vs[k], 0));
+        }
 }
 
 // Workgroups of a call: one for each row where rows are short, or else as many shares as
@@ -569,17 +585,24 @@ extern "C" int32_t locks_kv4_decode(
         a.shares = reinterpret_cast<int2*>(a.l + slots);
     }
     hipStream_t st = (hipStream_t)stream;
-#define KV4_LAUNCH(KERNEL, grid)                                                                                  \
-    do {                                                                                                          \
-        if (head_dim == 64) hipLaunchKernelGGL(KERNEL<64>, dim3((unsigned)(grid)), dim3(K4_BLK), 0, st, a);       \
-        else if (head_dim == 128) hipLaunchKernelGGL(KERNEL<128>, dim3((unsigned)(grid)), dim3(K4_BLK), 0, st, a); \
-        else hipLaunchKernelGGL(KERNEL<256>, dim3((unsigned)(grid)), dim3(K4_BLK), 0, st, a);                     \
-    } while (0)
-    KV4_LAUNCH(kv4_decode_kernel, wgs);
+    if (head_dim == 64) hipLaunchKernelGGL(kv4_decode_kernel<64>, dim3((unsigned)wgs), dim3(K4_BLK), 0, st, a);
+    else if (head_dim == 128) hipLaunchKernelGGL(kv4_decode_kernel<128>, dim3((unsigned)wgs), dim3(K4_BLK), 0, st, a);
+    else hipLaunchKernelGGL(kv4_decode_kernel<256>, dim3((unsigned)wgs), dim3(K4_BLK), 0, st, a);
     rc = check_launch("kv4_decode_kernel");
     if (rc || a.rows) return rc;
-    KV4_LAUNCH(kv4_merge_kernel, (int64_t)n_req * n_kv * G);
-#undef KV4_LAUNCH
+    // heads of a workgroup of the merge: with 256 rows or more they fill the card together
+    int hpw = 1;
+    while ((int64_t)n_req * n_kv >= 256 && hpw < G && 2 * hpw * (head_dim / 4) <= K4_BLK) hpw *= 2;
+    const dim3 grid((unsigned)((int64_t)n_req * n_kv * ((G + hpw - 1) / hpw)));
+#define KV4_MERGE(D)                                                                                        \
+    do {                                                                                                    \
+        if (hpw == 1) hipLaunchKernelGGL((kv4_merge_kernel<D, true>), grid, dim3(K4_BLK), 0, st, a, 1);     \
+        else hipLaunchKernelGGL((kv4_merge_kernel<D, false>), grid, dim3(K4_BLK), 0, st, a, hpw);           \
+    } while (0)
+    if (head_dim == 64) KV4_MERGE(64);
+    else if (head_dim == 128) KV4_MERGE(128);
+    else KV4_MERGE(256);
+#undef KV4_MERGE
     return check_launch("kv4_merge_kernel");
 }
 
@@ -599,14 +622,24 @@ extern "C" int32_t locks_kv4_read(
                   "%s: the outputs must be 16-byte aligned, the slots 8-byte", what);
     if (n_tokens == 0) return 0;
     const long units = (long)n_tokens * n_kv * (head_dim / 8);
-    LOCKS_REQUIRE((units + 255) / 256 <= 0x7fffffffL, "%s: too many tokens and heads for one launch", what);
+    // four units a thread where that leaves two workgroups a CU and more (8272 tokens of 8
+    // heads 11.5 -> 9.7 us), or else one (112 tokens 2.7 us, with four 3.5)
+    const int per = units >= 256 * 4 * 512 ? 4 : 1;
+    const long wgs = (units + 256 * per - 1) / (256 * per);
+    LOCKS_REQUIRE(wgs <= 0x7fffffffL, "%s: too many tokens and heads for one launch", what);
     const Kv4ReadArgs a{cache, c_stride_block, c_stride_head, slots, k_out, k_stride_tok, k_stride_head, v_out,
                         v_stride_tok, v_stride_head, (long)num_blocks * page, units, n_kv,
                         page == 16 ? 4 : page == 32 ? 5 : 6};
-    const dim3 grid((unsigned)((units + 255) / 256));
+    const dim3 grid((unsigned)wgs);
     hipStream_t st = (hipStream_t)stream;
-    if (head_dim == 64) hipLaunchKernelGGL(kv4_read_kernel<64>, grid, dim3(256), 0, st, a);
-    else if (head_dim == 128) hipLaunchKernelGGL(kv4_read_kernel<128>, grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL(kv4_read_kernel<256>, grid, dim3(256), 0, st, a);
+#define KV4_READ(D)                                                                             \
+    do {                                                                                        \
+        if (per == 4) hipLaunchKernelGGL((kv4_read_kernel<D, 4>), grid, dim3(256), 0, st, a);   \
+        else hipLaunchKernelGGL((kv4_read_kernel<D, 1>), grid, dim3(256), 0, st, a);            \
+    } while (0)
+    if (head_dim == 64) KV4_READ(64);
+    else if (head_dim == 128) KV4_READ(128);
+    else KV4_READ(256);
+#undef KV4_READ
     return check_launch("kv4_read_kernel");
 }
