@@ -95,14 +95,17 @@ __device__ __forceinline__ double wave_incl_scan(double v) {
 __device__ __forceinline__ uint32_t lows(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x05040100u); }
 __device__ __forceinline__ uint32_t highs(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
 
-template <int D>
-__global__ __launch_bounds__(K4_BLK, 2) void kv4_decode_kernel(const Kv4DecodeArgs a)
+// WV waves: 4, or 8 where a workgroup has a row and a CU to itself (a step is some 260
+// instructions one after the other, 1 us for a wave alone on its SIMD).
+template <int D, int WV>
+__global__ __launch_bounds__(WV * kWave, WV == 4 ? 2 : 1) void kv4_decode_kernel(const Kv4DecodeArgs a)
 {
+    constexpr int BLK = WV * kWave;
     using L = Kv4<D>;
     constexpr int ND = D / 16, W = L::W, T = K4_TILES;
-    __shared__ float m_s[K4_WAVES][16], l_s[K4_WAVES][16];
-    __shared__ __attribute__((aligned(16))) float o_s[K4_WAVES][16][D + 4];
-    __shared__ double sum_s[K4_WAVES];
+    __shared__ float m_s[WV][16], l_s[WV][16];
+    __shared__ __attribute__((aligned(16))) float o_s[WV][16][D + 4];
+    __shared__ double sum_s[WV];
     __shared__ long at_s[2];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int c16 = lane & 15, kg = lane >> 4;
@@ -129,7 +132,7 @@ __global__ __launch_bounds__(K4_BLK, 2) void kv4_decode_kernel(const Kv4DecodeAr
             r = __ffsll(__ballot(inc > (double)lo)) - 1;
             start = uniform((long)__shfl(inc - cost, r));
         } else {
-            const int per = (a.n_req + K4_BLK - 1) / K4_BLK;       // consecutive requests of a thread
+            const int per = (a.n_req + BLK - 1) / BLK;       // consecutive requests of a thread
             const int r0 = min(tid * per, a.n_req), r1 = min(r0 + per, a.n_req);
             double mine = 0.0;
             for (int i = r0; i < r1; ++i) mine += (double)Kv4Row(a, a.seq_lens[i]).cost() * a.n_kv;
@@ -137,7 +140,7 @@ __global__ __launch_bounds__(K4_BLK, 2) void kv4_decode_kernel(const Kv4DecodeAr
             if (lane == 63) sum_s[wave] = inc;
             __syncthreads();
             double before = inc - mine, all = 0.0;
-            for (int w = 0; w < K4_WAVES; ++w) {
+            for (int w = 0; w < WV; ++w) {
                 before += w < wave ? sum_s[w] : 0.0;
                 all += sum_s[w];
             }
@@ -195,16 +198,16 @@ __global__ __launch_bounds__(K4_BLK, 2) void kv4_decode_kernel(const Kv4DecodeAr
         }
     }
 
-    // step `it` of this wave: tiles n0 + T (wave + K4_WAVES it) .., T of them.  Addresses
+    // step `it` of this wave: tiles n0 + T (wave + WV it) .., T of them.  Addresses
     // and first keys of 64 tiles are made at once, one per lane.
     const int mine = n0 + T * wave;
-    const int steps = n1 > mine ? (n1 - mine + T * K4_WAVES - 1) / (T * K4_WAVES) : 0;
+    const int steps = n1 > mine ? (n1 - mine + T * WV - 1) / (T * WV) : 0;
     uint32_t at_lo = 0, at_hi = 0;
     int key_of = 0, it_of = 0;
     uint64_t edges = 0;
     auto fetch = [&](int it) __attribute__((always_inline)) {
         it_of = it;
-        const int n = mine + T * (K4_WAVES * (it + lane / T)) + lane % T, nc = min(n, n1 - 1);
+        const int n = mine + T * (WV * (it + lane / T)) + lane % T, nc = min(n, n1 - 1);
         const int tile = nc < na ? nc : b0 + nc - na;
         const int id = a.bt[(long)r * a.bt_sr + min(tile >> (a.pg_sh - 4), a.bt_cols - 1)];
         const uint64_t at = (uint64_t)a.c + (uint64_t)((long)min(max(id, 0), a.NB - 1) * a.c_sb + (long)kh * a.c_sh +
@@ -357,14 +360,14 @@ __global__ __launch_bounds__(K4_BLK, 2) void kv4_decode_kernel(const Kv4DecodeAr
                     make_float4(o[b][i], o[b + 1][i], o[b + 2][i], o[b + 3][i]);
     }
     __syncthreads();
-    for (int u = tid; u < G * (D / 4); u += K4_BLK) {
+    for (int u = tid; u < G * (D / 4); u += BLK) {
         const int g = u / (D / 4), e = 4 * (u % (D / 4));
         float mm = -INFINITY, lt = 0.f;
 #pragma unroll
-        for (int w = 0; w < K4_WAVES; ++w) mm = fmaxf(mm, m_s[w][g]);
+        for (int w = 0; w < WV; ++w) mm = fmaxf(mm, m_s[w][g]);
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int w = 0; w < K4_WAVES; ++w) {
+        for (int w = 0; w < WV; ++w) {
             const float lw = l_s[w][g];
             if (lw == 0.f) continue;                // a wave without keys
             const float f = mm == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_s[w][g] - mm);
@@ -529,7 +532,11 @@ __global__ __launch_bounds__(256) void kv4_read_kernel(const Kv4ReadArgs a)
 
 // Workgroups of a call: one for each row where rows are short, or else as many shares as
 // the card holds at once.
-static bool kv4_rows(int n_req, int n_kv, long max_keys) { return max_keys <= 512; }
+// (a row of its own for each workgroup: 49 requests of up to 936 tokens 11.8 -> 9.4 us, 32 of 2000
+// 22.0 -> 18.7, but one of 2000 10.8 -> 16.7)
+static bool kv4_rows(int n_req, int n_kv, long max_keys) {
+    return max_keys <= 1024 || (max_keys <= 2048 && (long)n_req * n_kv >= 256);
+}
 int64_t kv4_workspace(int n_req, int n_kv, int G, int head_dim) {
     return (int64_t)K4_GRID * 2 * G * (head_dim + 2) * 4 + (int64_t)n_req * n_kv * 8;
 }
@@ -585,9 +592,16 @@ extern "C" int32_t locks_kv4_decode(
         a.shares = reinterpret_cast<int2*>(a.l + slots);
     }
     hipStream_t st = (hipStream_t)stream;
-    if (head_dim == 64) hipLaunchKernelGGL(kv4_decode_kernel<64>, dim3((unsigned)wgs), dim3(K4_BLK), 0, st, a);
-    else if (head_dim == 128) hipLaunchKernelGGL(kv4_decode_kernel<128>, dim3((unsigned)wgs), dim3(K4_BLK), 0, st, a);
-    else hipLaunchKernelGGL(kv4_decode_kernel<256>, dim3((unsigned)wgs), dim3(K4_BLK), 0, st, a);
+    const bool wide = a.rows && wgs <= 256;
+#define KV4_DECODE(D)                                                                                                    \
+    do {                                                                                                                 \
+        if (wide) hipLaunchKernelGGL((kv4_decode_kernel<D, 8>), dim3((unsigned)wgs), dim3(8 * kWave), 0, st, a);         \
+        else hipLaunchKernelGGL((kv4_decode_kernel<D, K4_WAVES>), dim3((unsigned)wgs), dim3(K4_BLK), 0, st, a);          \
+    } while (0)
+    if (head_dim == 64) KV4_DECODE(64);
+    else if (head_dim == 128) KV4_DECODE(128);
+    else KV4_DECODE(256);
+#undef KV4_DECODE
     rc = check_launch("kv4_decode_kernel");
     if (rc || a.rows) return rc;
     // heads of a workgroup of the merge: with 256 rows or more they fill the card together
