@@ -213,7 +213,7 @@ __global__ __launch_bounds__(QK_BLK) void qkv_write_kernel(const QkvArgs a)
 // and the sum 4, the subtraction below 1); with twice that and more, 2^-19, on either side
 // the code is mostly the same, and only the heads of a wave with a value in doubt (one
 // wave of 50 to 100) go to 64 bits.  8192 tokens of 48 heads: all in 64 bits 54.6 us, so
-// 48.5, without rounding keys at all 41.
+// 48.5 (three groups a wave; 43.1 with six), without rounding keys at all 41.
 template <int D>
 __device__ __forceinline__ double head_sum(double s) {
 #pragma unroll
@@ -601,14 +601,18 @@ int32_t launch_qkv(QkvArgs a, bool kv4, int head_dim, int interleaved, int weigh
     auto grid_of = [&](int it) { return dim3((unsigned)(((long)a.n_tok * cdiv(a.groups, it) + QK_WAVES - 1) / QK_WAVES)); };
     const dim3 grid = grid_of(IT);
     a.w_f32 = weights_f32;
-    // The staged kernel: a call of one group per wave and at most two waves a SIMD is as
-    // long as one wave (32 tokens of 12 groups, along three axes 4.7 -> 3.6 us; 512
-    // tokens 5.9 -> 6.6)
-    const bool one = (long)a.n_tok * a.groups <= 2048;
-    const dim3 grid1 = grid_of(1);
-#define LAUNCH_S(DV, INTER, AXES, KV4)                                                                                  \
-    if (one) hipLaunchKernelGGL((qkv_staged_kernel<DV, 1, INTER, AXES, KV4>), grid1, dim3(QK_BLK), 0, st, a);           \
-    else hipLaunchKernelGGL((qkv_staged_kernel<DV, IT, INTER, AXES, KV4>), grid, dim3(QK_BLK), 0, st, a)
+    // The staged kernel.  One group per wave up to two waves a SIMD, where a call is as
+    // long as one wave (32 tokens of 12 groups, along three axes 4.7 -> 3.6 us; 512 tokens
+    // 5.9 -> 6.6); six where many workgroups follow each other on a CU and their starts
+    // (positions, angles, barrier) count (8192 tokens, into 4 bits 48.3 -> 43.1; 4097 of an
+    // image encoder 13.6 -> 11.7; 512 tokens 5.9 -> 7.0).
+    const long units = (long)a.n_tok * a.groups;
+    const int it = units <= 2048 ? 1 : units < 16384 ? IT : 6;
+    const dim3 grid_s = grid_of(it);
+#define LAUNCH_S(DV, INTER, AXES, KV4)                                                                                   \
+    if (it == 1) hipLaunchKernelGGL((qkv_staged_kernel<DV, 1, INTER, AXES, KV4>), grid_s, dim3(QK_BLK), 0, st, a);       \
+    else if (it == IT) hipLaunchKernelGGL((qkv_staged_kernel<DV, IT, INTER, AXES, KV4>), grid_s, dim3(QK_BLK), 0, st, a); \
+    else hipLaunchKernelGGL((qkv_staged_kernel<DV, 6, INTER, AXES, KV4>), grid_s, dim3(QK_BLK), 0, st, a)
 #define LAUNCH_W(DV, INTER)                                                                                             \
     if (kv4 && a.n_axes) { LAUNCH_S(DV, INTER, true, true); }                                                           \
     else if (kv4) { LAUNCH_S(DV, INTER, false, true); }                                                                 \

@@ -537,3 +537,109 @@ def test_c_entry_refusals():
                 dict(cb=40), dict(q=0), dict(qst=4), dict(H=5000), dict(eps=-1.0), dict(n=-1), dict(slot=0)):
         assert lib.locks_kv4_write(*{**ok, **bad}.values()) == -1, bad
         assert lib.locks_last_error().startswith(b"locks_kv4_write")
+
+
+# ---- calls at the edges of what is allowed ------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [65, 300, 700])
+@pytest.mark.parametrize("window, sinks", [(0, 0), (2500, 7)])
+def test_decode_more_requests_than_lanes(n, window, sinks):
+    """Shares over more requests than a wave has lanes, and than a workgroup has threads; many
+    of them without a token."""
+    g = torch.Generator()
+    g.manual_seed(n)
+    lens = [int(x) if i % 7 else 0 for i, x in enumerate(torch.randint(1, 200, (n,), generator=g))]
+    lens[3], lens[n // 2], lens[-1] = 2900, 1333, 2100
+    c = case(lens, [1] * n, 2, 2, 64, 16, width=190)
+    _agree(*_decode(c, window, sinks), _empty_row(c, _exact(_no_rows(c), window, sinks)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d, G", [(64, 7), (128, 1), (128, 16), (256, 3)])
+def test_decode_short_rows_of_a_wide_table(d, G):
+    """A table for far more tokens than there are: few shares, rows in one of them or cut
+    anywhere; no tokens at all."""
+    for lens in ([1], [33], [900], [17, 0, 1], [0, 0], [500, 1, 700, 64, 16], [2000] * 9):
+        c = case(lens, [1] * len(lens), 3, G, d, 16, width=4000, seed=len(lens))
+        want = _empty_row(c, _exact(_no_rows(c), 0, 0)) if any(lens) else None
+        out, lse = _decode(c)
+        if want is None:
+            assert not bool(out.any()) and bool((lse == -torch.inf).all())
+        else:
+            _agree(out, lse, want)
+
+
+@pytest.mark.gpu
+def test_prefill_many_requests_and_table_ends():
+    """More requests than lanes, some without a token; rows past the table's end see what
+    the table holds, or nothing where a window lies behind it."""
+    lens = [(37 * i) % 90 + 1 for i in range(150)]
+    new = [min(n, (11 * i) % 9) for i, n in enumerate(lens)]
+    c = case(lens, new, 2, 4, 128, 16)
+    _agree(*_prefill(c, 40, 3), _exact(c, 40, 3))
+    c = case([900], [900], 2, 4, 64, 16, width=30)                  # 480 tokens of the table
+    out, lse = _prefill(c, 100)
+    k, v = c["k"][0][:480], c["v"][0][:480]
+    head = {**c, "lens": [480], "new": [480], "q": c["q"][:480], "k": [k], "v": [v]}
+    _agree(out[:480], lse[:480], _exact(head, 100, 0))
+    assert not bool(out[579:].any()) and bool((lse[579:] == -torch.inf).all())
+
+
+@pytest.mark.gpu
+def test_in_place():
+    """q_out is q and k_out is k, views of one packed projection; fewer tokens than rows."""
+    x = inputs(70, 8, 2, 128, 128, 3)
+    axes = RopeAxes.sections((16, 24, 24))
+    one, two = (_blank(x["blocks"], 2, 128, 16) for _ in range(2))
+    q, k = torch.zeros_like(x["q"]), torch.zeros_like(x["k"])
+    kw = dict(q_weight=x["qw"], k_weight=x["kw"], axes=axes, n_tokens=64)
+    qk_norm_rope_write(x["q"], x["k"], x["v"], x["pos"], x["slots"], one, x["cs"], q, k_out=k, **kw)
+    packed = torch.cat([x["q"], x["k"], x["v"]], 1)
+    qp, kp, vp = packed.split([8, 2, 2], dim=1)
+    qk_norm_rope_write(qp, kp, vp, x["pos"], x["slots"], two, x["cs"], qp, k_out=kp, **kw)
+    assert torch.equal(one, two) and torch.equal(q[:64], qp[:64]) and torch.equal(k[:64], kp[:64])
+    assert torch.equal(qp[64:], x["q"][64:]) and not bool(q[64:].any())
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits():
+    """A cache of more than 4 GiB, its last pages in use."""
+    n_kv, d, page, blocks = 8, 128, 16, 250001
+    cache = kv4_cache(blocks, n_kv=n_kv, head_dim=d, page=page, device="cuda")
+    assert cache.nbytes > 1 << 32
+    g = torch.Generator(device="cuda")
+    g.manual_seed(1)
+    pages = torch.tensor([blocks - 1, 3, blocks - 77, 130000, 249000], device="cuda")
+    t = torch.arange(75, device="cuda")
+    slots = pages[t // page] * page + t % page
+    k, v = (torch.randn(75, n_kv, d, generator=g, device="cuda").to(torch.bfloat16) for _ in range(2))
+    qk_norm_rope_write(k, k, v, t.int(), slots, cache, None, torch.empty_like(k))
+    kr, vr = _read(cache, slots)
+    assert torch.equal(kr.double(), quantised(k.double())[2]) and torch.equal(vr.double(), quantised(v.double())[2])
+    c = dict(q=torch.randn(75, 16, d, generator=g, device="cuda").to(torch.bfloat16), kv=cache, bt=pages[None].int().contiguous(),
+             sl=torch.tensor([75], dtype=torch.int32, device="cuda"), qsl=torch.tensor([0, 75], dtype=torch.int32, device="cuda"),
+             k=[kr], v=[vr], lens=[75], new=[75], n_kv=n_kv, G=2, d=d, page=page, scale=0.1)
+    _agree(*_prefill(c), _exact(c, 0, 0))
+    one = {**c, "q": c["q"][:1].contiguous(), "new": [1]}
+    _agree(*_decode(one), _exact(one, 0, 0))
+
+
+@pytest.mark.gpu
+def test_replay_in_shares():
+    """A captured decode over a wide table follows the lengths: rows whole, cut and empty."""
+    n_kv, G, d = 2, 4, 128
+    c = case([2900, 1500, 40, 700], [1] * 4, n_kv, G, d, 16, width=200)
+    out, lse = _outs(c)
+    ws = _ws(c)
+    sl = c["sl"].clone()
+    call = lambda: window_decode(c["q"], c["kv"], c["bt"], sl, out, ws, n_req=4, scale=c["scale"], lse=lse)  # noqa: E731
+    call()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        call()
+    for lens in ([2900, 1500, 40, 700], [1, 2, 3, 4], [0, 1500, 0, 0], [2900, 0, 40, 699], [2048, 1499, 1, 16]):
+        sl.copy_(torch.tensor(lens, dtype=torch.int32))
+        g.replay()
+        part = {**c, "lens": lens, "k": [k[:n] for k, n in zip(c["k"], lens)], "v": [v[:n] for v, n in zip(c["v"], lens)]}
+        _agree(out, lse, _empty_row(part, _exact(_no_rows(part), 0, 0)))
+        torch.cuda.synchronize()
