@@ -39,7 +39,7 @@ struct QkvArgs {
     long slots;                             // num_blocks * page
     int max_pos, rot, n_tok, H, n_kv, pg_sh, groups;
     float eps;
-    // AXES: positions of n_axes axes, pos_ax apart, and each pair's axis in two bits
+    // staged: positions of n_axes axes, pos_ax apart, and each pair's axis in two bits
     int n_axes; long pos_ax;
     uint64_t axes[4];
     int w_f32;
@@ -295,13 +295,13 @@ __device__ __forceinline__ uint32_t to_codes(const uint4& raw, uint32_t& byte) {
     return codes8(y);
 }
 
-// Heads whose pairs turn by several axes' positions (AXES), or that go to a cache in 4
-// bits (KV4).  As above, but what a token's heads share stands in LDS, in fp32: its
+// Heads whose pairs turn by several axes' positions, or that go to a cache in 4 bits (KV4,
+// with one axis or more).  As above, but what a token's heads share stands in LDS, in fp32: its
 // angles, put together from every axis' row once, and the weights.  A lane reads what
 // it needs of them where it needs it, which leaves the registers to the rows on their
 // way and to the keys' doubles.
 constexpr int QK_TOK = QK_WAVES;            // tokens that a workgroup's waves may stand in
-template <int D, int IT, bool INTER, bool AXES, bool KV4>
+template <int D, int IT, bool INTER, bool KV4>
 __global__ __launch_bounds__(QK_BLK) void qkv_staged_kernel(const QkvArgs a)
 {
     constexpr int LPH = D / 8, HPW = kWave / LPH;
@@ -333,11 +333,10 @@ __global__ __launch_bounds__(QK_BLK) void qkv_staged_kernel(const QkvArgs a)
                                              : a.v + (long)t * a.v_st + (long)(x - a.H - a.n_kv) * a.v_sh;
         raw[i] = __builtin_bit_cast(uint4, __builtin_nontemporal_load(reinterpret_cast<const v4i*>(p + e0)));
     }
-    const int axes = AXES ? a.n_axes : 1;
     bool placed = true;
 #pragma unroll
-    for (int x = 0; x < (AXES ? QK_AXES : 1); ++x) {
-        const int pos = a.pos[t + (AXES ? min(x, axes - 1) * a.pos_ax : 0)];
+    for (int x = 0; x < QK_AXES; ++x) {
+        const int pos = a.pos[t + min(x, a.n_axes - 1) * a.pos_ax];
         placed = placed && pos >= 0 && pos < a.max_pos;
     }
     const long slot = a.slot[t];
@@ -346,11 +345,8 @@ __global__ __launch_bounds__(QK_BLK) void qkv_staged_kernel(const QkvArgs a)
     const int t1 = min((int)((unit0 + QK_WAVES - 1) / chunks), a.n_tok - 1);
     for (int i = tid; i < (t1 - t0 + 1) * a.rot; i += QK_BLK) {
         const int tt = i / a.rot, j = i - tt * a.rot, pair = j < half ? j : j - half;
-        int x = 0;
-        if constexpr (AXES) {
-            const uint64_t w = pair < 32 ? a.axes[0] : pair < 64 ? a.axes[1] : pair < 96 ? a.axes[2] : a.axes[3];
-            x = (int)(w >> (2 * (pair & 31)) & 3);
-        }
+        const uint64_t w = pair < 32 ? a.axes[0] : pair < 64 ? a.axes[1] : pair < 96 ? a.axes[2] : a.axes[3];
+        const int x = (int)(w >> (2 * (pair & 31)) & 3);
         const int pos = a.pos[t0 + tt + x * a.pos_ax];
         ang_s[tt][j] = a.cs[(long)(pos >= 0 && pos < a.max_pos ? pos : 0) * a.rot + j];
     }
@@ -609,14 +605,13 @@ int32_t launch_qkv(QkvArgs a, bool kv4, int head_dim, int interleaved, int weigh
     const long units = (long)a.n_tok * a.groups;
     const int it = units <= 2048 ? 1 : units < 16384 ? IT : 6;
     const dim3 grid_s = grid_of(it);
-#define LAUNCH_S(DV, INTER, AXES, KV4)                                                                                   \
-    if (it == 1) hipLaunchKernelGGL((qkv_staged_kernel<DV, 1, INTER, AXES, KV4>), grid_s, dim3(QK_BLK), 0, st, a);       \
-    else if (it == IT) hipLaunchKernelGGL((qkv_staged_kernel<DV, IT, INTER, AXES, KV4>), grid_s, dim3(QK_BLK), 0, st, a); \
-    else hipLaunchKernelGGL((qkv_staged_kernel<DV, 6, INTER, AXES, KV4>), grid_s, dim3(QK_BLK), 0, st, a)
+#define LAUNCH_S(DV, INTER, KV4)                                                                                   \
+    if (it == 1) hipLaunchKernelGGL((qkv_staged_kernel<DV, 1, INTER, KV4>), grid_s, dim3(QK_BLK), 0, st, a);       \
+    else if (it == IT) hipLaunchKernelGGL((qkv_staged_kernel<DV, IT, INTER, KV4>), grid_s, dim3(QK_BLK), 0, st, a); \
+    else hipLaunchKernelGGL((qkv_staged_kernel<DV, 6, INTER, KV4>), grid_s, dim3(QK_BLK), 0, st, a)
 #define LAUNCH_W(DV, INTER)                                                                                             \
-    if (kv4 && a.n_axes) { LAUNCH_S(DV, INTER, true, true); }                                                           \
-    else if (kv4) { LAUNCH_S(DV, INTER, false, true); }                                                                 \
-    else if (a.n_axes) { LAUNCH_S(DV, INTER, true, false); }                                                            \
+    if (kv4) { LAUNCH_S(DV, INTER, true); }                                                                             \
+    else if (a.n_axes) { LAUNCH_S(DV, INTER, false); }                                                                  \
     else if (weights_f32) hipLaunchKernelGGL((qkv_write_kernel<DV, IT, INTER, true>), grid, dim3(QK_BLK), 0, st, a);    \
     else hipLaunchKernelGGL((qkv_write_kernel<DV, IT, INTER, false>), grid, dim3(QK_BLK), 0, st, a)
 #define LAUNCH(DV)                              \
@@ -681,6 +676,7 @@ extern "C" int32_t locks_kv4_write(
     if (rc) return rc;
     rc = check_axes(what, a, n_axes, pos_stride_axis, {axes0, axes1, axes2, axes3});
     if (rc) return rc;
+    a.n_axes = n_axes ? n_axes : 1;         // one position: one axis, all words 0
     return launch_qkv(a, true, head_dim, interleaved, weights_f32, (hipStream_t)stream);
 }
 
