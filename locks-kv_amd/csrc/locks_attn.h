@@ -68,11 +68,6 @@ inline long bound_keys(int32_t max_seq_len, int32_t bt_cols, int32_t page) {
 }
 
 
-// Joins the partials of every row (locks_window.hip); with `starts` only of the rows
-// of starts[0] .. starts[n_seq].
-int launch_merge(const Partials& p, uint16_t* out, long o_st, long o_sh, float* lse, long lse_st, int n_tok, int n_kv,
-                 int G, int head_dim, const int* starts, int n_seq, hipStream_t st);
-
 // Bytes of a call's partials, and where they stand in its workspace.
 inline int64_t part_bytes(int64_t rows, int splits, int D) { return rows * splits * (D + 2) * 4; }
 inline Partials part_layout(void* ws, int64_t rows, int splits, int D) {

@@ -111,4 +111,17 @@ __device__ __forceinline__ uint4 kv4_eight(uint32_t w, float scale) {
     return make_uint4(kv4_pair<0>(w, scale), kv4_pair<1>(w, scale), kv4_pair<2>(w, scale), kv4_pair<3>(w, scale));
 }
 
+// What kv4_merge_kernel joins: partials m (the maximum, as a base-2 logarithm of the
+// weight), l and acc, of a row's shares, or of its `splits`.
+struct Kv4MergeArgs {
+    const float* m; const float* l; const float* acc;
+    const int2* shares;                     // or null: splits
+    int splits;
+    const int* starts; int n_seq;           // splits: the requests' first tokens
+    uint16_t* out; long o_sr, o_sh;
+    float* lse; long lse_sr;
+    int n_kv, G;
+};
+int launch_kv4_merge(const Kv4MergeArgs& a, int n_rows, int head_dim, hipStream_t st);
+
 }  // namespace locks

@@ -396,13 +396,14 @@ __global__ __launch_bounds__(WV * kWave, WV == 4 ? 2 : 1) void kv4_decode_kernel
     }
 }
 
-// Joins the shares of every row that has several: `hpw` heads of a row a workgroup (all
+// Joins the partials of every row that has several: `hpw` heads of a row a workgroup (all
 // that fit where there are many rows, one where there are few), D / 4 columns each, and
-// what threads are left as streams over the shares.  The first share's partial is in its
-// second slot (it starts the row), the others' in their first.
+// what threads are left as streams over the partials.  A decode's row has those of its
+// shares, the first one's in its second slot (it starts the row), the others' in their
+// first; a prompt's row (SHARES false) one of each split.
 constexpr int K4_GRID = 512;                // shares at most: two workgroups a CU
-template <int D, bool ONE>
-__global__ __launch_bounds__(K4_BLK) void kv4_merge_kernel(const Kv4DecodeArgs a, int heads)
+template <int D, bool ONE, bool SHARES>
+__global__ __launch_bounds__(K4_BLK) void kv4_merge_kernel(const Kv4MergeArgs a, int heads)
 {
     const int hpw = ONE ? 1 : heads;
     constexpr int COLS = D / 4, PF = 8;
@@ -412,9 +413,17 @@ __global__ __launch_bounds__(K4_BLK) void kv4_merge_kernel(const Kv4DecodeArgs a
     const int hh = tid / COLS % hpw, strm = tid / (COLS * hpw), streams = K4_BLK / (COLS * hpw);
     const long row = blockIdx.x / n_heads;          // request, kv head
     const int g = blockIdx.x % n_heads * hpw + hh;
-    const int2 sh = a.shares[row];
-    const int n = sh.y - sh.x + 1;
-    if (n <= 0) return;
+    int2 sh = make_int2(0, 0);
+    int n = a.splits;
+    if constexpr (SHARES) {
+        sh = a.shares[row];
+        n = sh.y - sh.x + 1;
+        if (n <= 0) return;
+    } else {
+        // rows before the first request or after the last one have no partials
+        const long t = row / a.n_kv;
+        if (t < a.starts[0] || t >= a.starts[a.n_seq]) return;
+    }
     const bool mine = strm < streams && g < a.G;
     // the running maximum, sum and columns over this stream's shares
     float m = -INFINITY, l = 0.f;
@@ -425,7 +434,7 @@ __global__ __launch_bounds__(K4_BLK) void kv4_merge_kernel(const Kv4DecodeArgs a
 #pragma unroll
         for (int k = 0; k < PF; ++k) {
             const int i = min(i0 + k * streams, n - 1);
-            const long at = (2L * (sh.x + i) + (i == 0)) * a.G + g;
+            const long at = (SHARES ? 2L * (sh.x + i) + (i == 0) : row * n + i) * a.G + g;
             mi[k] = a.m[at];
             li[k] = i0 + k * streams < n ? a.l[at] : 0.f;
             x[k] = *reinterpret_cast<const float4*>(a.acc + at * D + 4 * col);
@@ -530,6 +539,31 @@ __global__ __launch_bounds__(256) void kv4_read_kernel(const Kv4ReadArgs a)
         }
 }
 
+int launch_kv4_merge(const Kv4MergeArgs& a, int n_rows, int head_dim, hipStream_t st)
+{
+    // heads of a workgroup: with 256 rows or more they fill the card together
+    const int64_t rows = (int64_t)n_rows * a.n_kv;
+    int hpw = 1;
+    while (rows >= 256 && hpw < a.G && 2 * hpw * (head_dim / 4) <= K4_BLK) hpw *= 2;
+    const dim3 grid((unsigned)(rows * ((a.G + hpw - 1) / hpw)));
+#define KV4_MERGE(D, SHARES)                                                                                          \
+    do {                                                                                                              \
+        if (hpw == 1) hipLaunchKernelGGL((kv4_merge_kernel<D, true, SHARES>), grid, dim3(K4_BLK), 0, st, a, 1);       \
+        else hipLaunchKernelGGL((kv4_merge_kernel<D, false, SHARES>), grid, dim3(K4_BLK), 0, st, a, hpw);             \
+    } while (0)
+#define KV4_MERGE_D(D)                          \
+    do {                                        \
+        if (a.shares) KV4_MERGE(D, true);       \
+        else KV4_MERGE(D, false);               \
+    } while (0)
+    if (head_dim == 64) KV4_MERGE_D(64);
+    else if (head_dim == 128) KV4_MERGE_D(128);
+    else KV4_MERGE_D(256);
+#undef KV4_MERGE_D
+#undef KV4_MERGE
+    return check_launch("kv4_merge_kernel");
+}
+
 // Workgroups of a call: one for each row where rows are short, or else as many shares as
 // the card holds at once.
 // (a row of its own for each workgroup: 49 requests of up to 936 tokens 11.8 -> 9.4 us, 32 of 2000
@@ -604,20 +638,8 @@ extern "C" int32_t locks_kv4_decode(
 #undef KV4_DECODE
     rc = check_launch("kv4_decode_kernel");
     if (rc || a.rows) return rc;
-    // heads of a workgroup of the merge: with 256 rows or more they fill the card together
-    int hpw = 1;
-    while ((int64_t)n_req * n_kv >= 256 && hpw < G && 2 * hpw * (head_dim / 4) <= K4_BLK) hpw *= 2;
-    const dim3 grid((unsigned)((int64_t)n_req * n_kv * ((G + hpw - 1) / hpw)));
-#define KV4_MERGE(D)                                                                                        \
-    do {                                                                                                    \
-        if (hpw == 1) hipLaunchKernelGGL((kv4_merge_kernel<D, true>), grid, dim3(K4_BLK), 0, st, a, 1);     \
-        else hipLaunchKernelGGL((kv4_merge_kernel<D, false>), grid, dim3(K4_BLK), 0, st, a, hpw);           \
-    } while (0)
-    if (head_dim == 64) KV4_MERGE(64);
-    else if (head_dim == 128) KV4_MERGE(128);
-    else KV4_MERGE(256);
-#undef KV4_MERGE
-    return check_launch("kv4_merge_kernel");
+    return launch_kv4_merge(Kv4MergeArgs{a.m, a.l, a.acc, a.shares, 0, nullptr, 0, out, out_stride_req, out_stride_head, lse,
+                                         lse_stride_req, n_kv, G}, n_req, head_dim, st);
 }
 
 extern "C" int32_t locks_kv4_read(

@@ -413,7 +413,7 @@ __global__ __launch_bounds__(P4_BLK, D == 256 ? 1 : 2) void kv4_prefill_kernel(c
     if constexpr (PART) {
         const long at = (((long)tok * a.n_kv + kh) * a.p.splits + sp) * G + g;
         if (h == 0) {
-            a.p.m[at] = l > 0.f || l != l ? m * a.scale : -INFINITY;
+            a.p.m[at] = l > 0.f || l != l ? m * a.scale_log2 : -INFINITY;
             a.p.l[at] = l;
         }
         float* ap = a.p.acc + at * D + 4 * h;
@@ -500,6 +500,6 @@ extern "C" int32_t locks_kv4_prefill(
 #undef P4_LAUNCH
     rc = check_launch("kv4_prefill_kernel");
     if (rc || ns == 1) return rc;
-    return launch_merge(a.p, out, out_stride_tok, out_stride_head, lse, lse_stride_tok, n_tokens, n_kv, G, head_dim,
-                        query_start_loc, n_req, st);
+    return launch_kv4_merge(Kv4MergeArgs{a.p.m, a.p.l, a.p.acc, nullptr, ns, query_start_loc, n_req, out, out_stride_tok,
+                                         out_stride_head, lse, lse_stride_tok, n_kv, G}, n_tokens, head_dim, st);
 }

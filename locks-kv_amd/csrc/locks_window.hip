@@ -641,7 +641,7 @@ static int shared_splits(long tiles, int n_kv, long max_keys, int head_dim) {
     return clampi((256 + wgs - 1) / wgs, 1, clampi(max_keys / (4 * kt), 1, 64));
 }
 
-int launch_merge(const Partials& p, uint16_t* out, long o_st, long o_sh, float* lse, long lse_st, int n_tok,
+static int launch_merge(const Partials& p, uint16_t* out, long o_st, long o_sh, float* lse, long lse_st, int n_tok,
                         int n_kv, int G, int head_dim, const int* starts, int n_seq, hipStream_t st) {
 #define LAUNCH_D(DV)                                                                                            \
     hipLaunchKernelGGL(attn_merge_kernel<DV>, dim3((unsigned)n_tok * n_kv * G), dim3(AM_BLK), 0, st, p, out, o_st, \
