@@ -192,18 +192,26 @@ _CALLS = {name: (i, _words(name)) for i, name in enumerate((
     "locks_kv4_prefill"))}
 
 
+_torch = None           # imported by the first launch: the statement costs 0.1 us in every call
+
+
 def launch(name: str, index: int, args: tuple) -> None:
     """Entry `name` with (*args, stream) on device `index` and its current stream,
     whichever device is the current one; raises where it refuses.  The arguments go
     as one block of words (locks_call)."""
-    import torch
+    global _torch
+    if _torch is None:
+        import torch
+        _torch = torch
     entry, packer = _CALLS[name]
-    call = load().locks_call
-    if index == torch._C._cuda_getDevice():
-        rc = call(entry, packer.pack(*args, stream_ptr(index)), len(args) + 1)
+    call = (_LIB or load()).locks_call
+    c = _torch._C
+    raw = getattr(c, "_cuda_getCurrentRawStream", None) or stream_ptr
+    if index == c._cuda_getDevice():
+        rc = call(entry, packer.pack(*args, raw(index)), len(args) + 1)
     else:
-        with torch.cuda.device(index):
-            rc = call(entry, packer.pack(*args, stream_ptr(index)), len(args) + 1)
+        with _torch.cuda.device(index):
+            rc = call(entry, packer.pack(*args, raw(index)), len(args) + 1)
     if rc:
         check(rc, name)
 
