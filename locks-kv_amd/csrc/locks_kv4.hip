@@ -24,7 +24,8 @@
 // merge: the chain of lengths, block ids and first tiles, and the join, are 10 of them); 32
 // requests of 1 to 32768 keys 54 us, 5.3 TB/s.  Two workgroups a CU, two steps on their
 // way: 70 KB a CU, more than latency x rate needs (three and four steps, and three
-// workgroups, were slower).  At d 64 the instructions of a step bound it (5.3 TB/s).
+// workgroups, were slower).  At d 64 the instructions of a step bound it: 1M keys 111 us,
+// 5.1 TB/s.
 #include "locks_attn.h"
 #include "locks_common.h"
 #include "locks_hip.h"
@@ -41,6 +42,14 @@ constexpr int K4_BLK = K4_WAVES * kWave;
 constexpr int K4_TILES = 2;                 // of a wave's step
 constexpr int K4_ROW = 32;                  // a row's start (query, first loads, output) in tiles' time
 constexpr int K4_SHARE = 24;                // tiles that a share has at least
+// Workgroups that a CU has registers for: at d 64 128 of them do (300 requests of 1500 keys
+// 56.1 us with three workgroups a CU, 51.3 with four).
+constexpr int kv4_resident(int head_dim) { return head_dim == 64 ? 4 : 2; }
+// Shares at most: two workgroups a CU, or three at d 64, where the instructions of a step
+// bound it (1M keys of 8 heads 122 -> 111 us, 64 requests of 4096 41.0 -> 37.5, 16 of 3000
+// 12.6 -> 13.0; four 110, 37.1 and 13.0).  Three cost more than they give at d 128 (131072
+// keys 33.2 -> 37.9 us) and where a group's partials are large (16 heads 19.7 -> 21.0).
+static int kv4_grid(int head_dim, int G) { return head_dim == 64 && G <= 8 ? 768 : 512; }
 constexpr float kLn2 = 0.69314718055994530942f;
 
 struct Kv4DecodeArgs {
@@ -105,7 +114,7 @@ __device__ __forceinline__ uint32_t highs(uint32_t a, uint32_t b) { return __bui
 // WV waves: 4, or 8 where a workgroup has a row and a CU to itself (a step is some 260
 // instructions one after the other, 1 us for a wave alone on its SIMD).
 template <int D, int WV>
-__global__ __launch_bounds__(WV * kWave, WV == 4 ? 2 : 1) void kv4_decode_kernel(const Kv4DecodeArgs a)
+__global__ __launch_bounds__(WV * kWave, WV == 4 ? kv4_resident(D) : 1) void kv4_decode_kernel(const Kv4DecodeArgs a)
 {
     constexpr int BLK = WV * kWave;
     using L = Kv4<D>;
@@ -176,6 +185,19 @@ __global__ __launch_bounds__(WV * kWave, WV == 4 ? 2 : 1) void kv4_decode_kernel
     }
 
     for (;;) {
+    // Q, asked for together with the row's length (one latency less: 500 keys 6.75 -> 6.61
+    // us): k-slots 8 kg .. of step st are entries kg D / 4 + 8 st ..
+    v8bf qf[W];
+    {
+        const uint16_t* qp = a.q + (long)r * a.q_sr + (long)(kh * G + c16) * a.q_sh + kg * (D / 4);
+#pragma unroll
+        for (int st = 0; st < W; ++st) {
+            uint4 w = make_uint4(0u, 0u, 0u, 0u);
+            if (c16 < G) w = *reinterpret_cast<const uint4*>(qp + 8 * st);
+            qf[st] = __builtin_bit_cast(v8bf, w);
+        }
+    }
+
     const Kv4Row row(a, uniform(a.seq_lens[r]));
     const int len = row.len, klo = row.lo, sinks = row.sinks, na = row.na, b0 = row.b0;
     const int units = max(row.nt, 1);
@@ -193,18 +215,6 @@ __global__ __launch_bounds__(WV * kWave, WV == 4 ? 2 : 1) void kv4_decode_kernel
     }
     n1 = min(n1, row.nt);
     if (work) {
-    // Q: k-slots 8 kg .. of step st are entries kg D / 4 + 8 st ..
-    v8bf qf[W];
-    {
-        const uint16_t* qp = a.q + (long)r * a.q_sr + (long)(kh * G + c16) * a.q_sh + kg * (D / 4);
-#pragma unroll
-        for (int st = 0; st < W; ++st) {
-            uint4 w = make_uint4(0u, 0u, 0u, 0u);
-            if (c16 < G) w = *reinterpret_cast<const uint4*>(qp + 8 * st);
-            qf[st] = __builtin_bit_cast(v8bf, w);
-        }
-    }
-
     // step `it` of this wave: tiles n0 + T (wave + WV it) .., T of them.  Addresses
     // and first keys of 64 tiles are made at once, one per lane.
     const int mine = n0 + T * wave;
@@ -408,7 +418,6 @@ __global__ __launch_bounds__(WV * kWave, WV == 4 ? 2 : 1) void kv4_decode_kernel
 // what threads are left as streams over the partials.  A decode's row has those of its
 // shares, the first one's in its second slot (it starts the row), the others' in their
 // first; a prompt's row (SHARES false) one of each split.
-constexpr int K4_GRID = 512;                // shares at most: two workgroups a CU
 template <int D, bool ONE, bool SHARES>
 __global__ __launch_bounds__(K4_BLK) void kv4_merge_kernel(const Kv4MergeArgs a, int heads)
 {
@@ -581,7 +590,7 @@ static bool kv4_rows(int n_req, int n_kv, long max_keys) {
     return max_keys <= 1024 || (max_keys <= 2048 && (long)n_req * n_kv >= 256);
 }
 int64_t kv4_workspace(int n_req, int n_kv, int G, int head_dim) {
-    return (int64_t)K4_GRID * 2 * G * (head_dim + 2) * 4 + (int64_t)n_req * n_kv * 8;
+    return (int64_t)kv4_grid(head_dim, G) * 2 * G * (head_dim + 2) * 4 + (int64_t)n_req * n_kv * 8;
 }
 
 int32_t check_kv4(const char* what, const void* cache, int64_t sb, int64_t sh, int32_t num_blocks, int32_t n_kv,
@@ -619,15 +628,16 @@ extern "C" int32_t locks_kv4_decode(
     if (n_req == 0) return 0;
     long keys = bound_keys(max_seq_len, bt_cols, page);
     if (window && (long)window + sinks + 32 < keys) keys = (long)window + sinks + 32;
+    const int shares = kv4_grid(head_dim, G);
     Kv4DecodeArgs a{q, q_stride_req, q_stride_head, cache, c_stride_block, c_stride_head, block_table, bt_stride, seq_lens,
                     out, out_stride_req, out_stride_head, lse, lse_stride_req, nullptr, nullptr, nullptr, nullptr,
-                    scale * kLog2e, 1.0 / K4_GRID, num_blocks, bt_cols, n_req, n_kv, G, page == 16 ? 4 : page == 32 ? 5 : 6, window, sinks,
-                    kv4_rows(n_req, n_kv, keys)};
+                    scale * kLog2e, 1.0 / shares, num_blocks, bt_cols, n_req, n_kv, G,
+                    page == 16 ? 4 : page == 32 ? 5 : 6, window, sinks, kv4_rows(n_req, n_kv, keys)};
     int wgs = n_req * n_kv;
     if (!a.rows) {
         rc = check_ws(what, workspace, workspace_bytes, kv4_workspace(n_req, n_kv, G, head_dim));
         if (rc) return rc;
-        wgs = K4_GRID;
+        wgs = shares;
         const int64_t slots = 2L * wgs * G;
         a.acc = static_cast<float*>(workspace);
         a.m = a.acc + slots * head_dim;
