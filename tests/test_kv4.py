@@ -570,6 +570,15 @@ def test_decode_short_rows_of_a_wide_table(d, G):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("d, G", [(64, 8), (64, 9), (64, 16), (128, 8), (256, 16)])
+@pytest.mark.parametrize("window, sinks", [(0, 0), (9000, 33)])
+def test_decode_full_grids_of_shares(d, G, window, sinks):
+    """Without a window every share of the grid has work, at each count of shares."""
+    c = case([20011, 3, 9007, 0, 12500], [1] * 5, 8, G, d, 32)
+    _agree(*_decode(c, window, sinks), _empty_row(c, _exact(_no_rows(c), window, sinks)))
+
+
+@pytest.mark.gpu
 def test_prefill_many_requests_and_table_ends():
     """More requests than lanes, some without a token; rows past the table's end see what
     the table holds, or nothing where a window lies behind it."""
