@@ -201,17 +201,19 @@ __global__ __launch_bounds__(P4_BLK, D == 256 ? 1 : 2) void kv4_prefill_kernel(c
         const int key0 = key_of(n);
         return key0 + KT > min_hi || (key0 < max_lo && key0 + KT > sinks);
     };
-    // NaN blocks of V in masked places must not reach the sums (0 x NaN).  In such a tile
-    // they are written as zeros, and noted: `nans` has a bit for each 32 columns that are
-    // NaN in a key that this lane's row sees.
+    // Blocks of V that are not finite must not reach the sums from masked places (0 x NaN):
+    // NaN ones, and those of scales past a write's (bytes 253 and 254 in memory that nobody
+    // wrote: 4 * 2^126 is infinite in bf16).  In such a tile they are written as zeros, and
+    // noted: `nans` has a bit for each 32 columns that are so in a key that this lane's row
+    // sees.
     auto clear_nan = [&](int n, Kv4Lane<D>& cv, int buf) __attribute__((always_inline)) {
-        const uint32_t z = ~cv.s;                       // a zero byte: a scale of 255
-        const bool any = __any(((z - 0x01010101u) & ~z & 0x80808080u) != 0);
+        // a byte of 253 and more: 0x7D and more below its top bit, which is set
+        const bool any = __any((((cv.s & 0x7F7F7F7Fu) + 0x03030303u) & cv.s & 0x80808080u) != 0);
         if (lane == 0) nan_s[buf][wave] = any;
         if (any && part(n)) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const bool bad = (cv.s >> (8 * i) & 255u) == 255u;
+                const bool bad = (cv.s >> (8 * i) & 255u) >= 253u;
                 if (r16 % (512 / D) == 0) nan_k[buf][16 * wave + 4 * kg + i][r16 / (512 / D)] = bad;
                 cv.s &= bad ? ~(255u << (8 * i)) : ~0u;
                 if constexpr (D == 64) cv.w[i >> 1] &= !bad ? ~0u : (i & 1) ? 0xFFFFu : 0xFFFF0000u;
