@@ -212,8 +212,13 @@ __global__ __launch_bounds__(QK_BLK) void qkv_write_kernel(const QkvArgs a)
 // pair's magnitude |a cos| + |b sin| (inverse root of the sum of squares 9, three products
 // and the sum 4, the subtraction below 1); with twice that and more, 2^-19, on either side
 // the code is mostly the same, and only the heads of a wave with a value in doubt (one
-// wave of 50 to 100) go to 64 bits.  8192 tokens of 48 heads: all in 64 bits 54.6 us, so
-// 48.5 (three groups a wave; 43.1 with six), without rounding keys at all 41.
+// wave of 50 to 100) go to 64 bits.  That holds where no product loses its bits below
+// fp32's normal numbers: a value next to a border is 2^-104 at least (of a block whose
+// largest is 2^-100, below which all is in doubt), and such a product is off by 2^-150,
+// times the weight and the angle behind it: less than 2^-127 with weights below 2^16 and
+// angles below 2^6, 2^-23 of the value.  Larger ones go to 64 bits.
+// 8192 tokens of 48 heads: all in 64 bits 54.6 us, so 48.5 (three groups a wave; 43.1
+// with six), without rounding keys at all 41.
 template <int D>
 __device__ __forceinline__ double head_sum(double s) {
 #pragma unroll
@@ -308,7 +313,7 @@ __global__ __launch_bounds__(QK_BLK) void qkv_staged_kernel(const QkvArgs a)
 {
     constexpr int LPH = D / 8, HPW = kWave / LPH;
     __shared__ __attribute__((aligned(16))) float ang_s[QK_TOK][D], w_s[2][D];
-    __shared__ int wild_s[QK_WAVES];        // a weight past 2^60: fp32 may lose a small entry under it
+    __shared__ int wild_s[QK_WAVES];        // a weight or an angle past what to_codes' bound allows
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int chunks = (a.groups + IT - 1) / IT;
     // KV4: 16 tokens share the lines of a tile.  Workgroups go round the 8 XCDs; of 128
@@ -344,22 +349,24 @@ __global__ __launch_bounds__(QK_BLK) void qkv_staged_kernel(const QkvArgs a)
     const long slot = a.slot[t];
     const int half = a.rot >> 1;
     // the angles of this workgroup's tokens, and the weights
+    bool big = false;
     const int t1 = min((int)((unit0 + QK_WAVES - 1) / chunks), a.n_tok - 1);
     for (int i = tid; i < (t1 - t0 + 1) * a.rot; i += QK_BLK) {
         const int tt = i / a.rot, j = i - tt * a.rot, pair = j < half ? j : j - half;
         const uint64_t w = pair < 32 ? a.axes[0] : pair < 64 ? a.axes[1] : pair < 96 ? a.axes[2] : a.axes[3];
         const int x = (int)(w >> (2 * (pair & 31)) & 3);
         const int pos = a.pos[t0 + tt + x * a.pos_ax];
-        ang_s[tt][j] = a.cs[(long)(pos >= 0 && pos < a.max_pos ? pos : 0) * a.rot + j];
+        const float y = a.cs[(long)(pos >= 0 && pos < a.max_pos ? pos : 0) * a.rot + j];
+        ang_s[tt][j] = y;
+        big = big || !(fabsf(y) < 0x1p6f);
     }
-    bool big = false;
     for (int i = tid; i < 2 * D; i += QK_BLK) {
         const void* w = i < D ? a.qw : a.kw;
         const int e = i % D;
         if (w) {
             const float x = a.w_f32 ? static_cast<const float*>(w)[e] : bf16_to_f32(static_cast<const uint16_t*>(w)[e]);
             w_s[i / D][e] = x;
-            big = big || !(fabsf(x) < 0x1p60f);
+            big = big || !(fabsf(x) < 0x1p16f);
         }
     }
     if (KV4) {
