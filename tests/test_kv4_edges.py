@@ -56,3 +56,80 @@ def test_large_weights_over_small_entries(weight, table, T, interleaved):
     _, _, want, near = quantised(k64)
     k, _ = _read(cache, x["slots"])
     assert torch.equal(torch.where(near, 0, k.double()), torch.where(near, 0, want)) and int(near.sum()) < 3
+
+
+def _put(c, request, key, k=None, v=None):
+    """Writes K and V of one key of a request again (heads of (n_kv, d)), others as they were."""
+    page = c["page"]
+    slot = c["bt"][request, key // page].long() * page + key % page
+    k = c["k"][request][key:key + 1] if k is None else k[None]
+    v = c["v"][request][key:key + 1] if v is None else v[None]
+    qk_norm_rope_write(k, k, v, slot[None].int() * 0, slot[None], c["kv"], None, torch.empty_like(k))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d, G", [(64, 8), (64, 5), (128, 4), (256, 2)])
+@pytest.mark.parametrize("where", [20, 300, 2900, 2955])
+def test_nan_values_in_split_prompts(d, G, where):
+    """A NaN block of V under a few new tokens of a long row, whose keys are split over
+    workgroups: in a tile that every row sees, one that the window's edge or the last rows
+    cut, and one of the sinks."""
+    n_kv = 2
+    c = case([3000, 2980], [50, 3], n_kv, G, d, 16, seed=where)
+    v = c["v"][0][where].clone()
+    v[1, d - 1] = torch.nan
+    _put(c, 0, where, v=v)
+    c["v"][0][where, 1, d - 32:] = torch.nan
+    for window, sinks in ((0, 0), (2660, 0), (100, 21), (47, 0), (2700, 300)):
+        _agree(*_prefill(c, window, sinks), _exact(c, window, sinks))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("lens, new", [([300, 300], [60, 7]), ([3000, 2000], [30, 7])])
+def test_nan_keys_in_prompts(d, lens, new):
+    """A written K block that is not finite: the rows that see it are NaN; it stands behind
+    the window of others, between it and the sinks, or past them."""
+    n_kv, G = 2, 4
+    c = case(lens, new, n_kv, G, d, 16)
+    n, m = lens[0], new[0]
+    for bad, value in ((n - m // 2, torch.nan), (n - 100, torch.inf), (10, -torch.inf)):
+        k = c["k"][0][bad].clone()
+        k[0, 33] = value
+        _put(c, 0, bad, k=k)
+        for window, sinks in ((0, 0), (90, 0), (90, 4), (90, 11), (m // 2, 10), (n, 0)):
+            out, lse = _prefill(c, window, sinks)
+            pos = torch.arange(n - m, n, device="cuda")
+            sees = (pos >= bad) & ((pos - bad < (window or n)) | (bad < sinks))
+            assert bool(out[:m][sees][:, :G].isnan().all()) and bool(lse[:m][sees][:, :G].isnan().all())
+            # the other rows and heads: as without the bad block
+            o, z, to, tz = _exact(c, window, sinks)
+            out[:m][sees, :G], lse[:m][sees, :G] = 0.0, 0.0
+            for x in (o, z, to, tz):
+                x[:m][sees, :G] = 0.0
+            _agree(out, lse, (o, z, to, tz))
+        _put(c, 0, bad)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_prompt_bounds_of_lengths(d):
+    """A bound of the lengths that is exact, and one that is too low, on a wide table: what
+    the call splits by, not what it attends to."""
+    c = case([2100, 5, 777], [9, 5, 200], 2, 4, d, 16, width=4000)
+    for window, sinks in ((0, 0), (700, 4)):
+        want = _exact(c, window, sinks)
+        for bound in (0, 2100, 300, 1):
+            _agree(*_prefill(c, window, sinks, max_seq_len=bound), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d, G", [(64, 8), (128, 4), (256, 4)])
+def test_the_same_call_twice(d, G):
+    """The same bits from the same call, whatever the workspace holds."""
+    c = case([9000, 40, 3000, 0, 700], [1] * 5, 2, G, d, 16)
+    p = case([9000, 40, 3000, 700], [30, 40, 1, 200], 2, G, d, 16)
+    for call, x in ((_decode, c), (_prefill, p)):
+        one = call(x)
+        for _ in range(3):
+            assert all(torch.equal(a, b) for a, b in zip(call(x), one))
