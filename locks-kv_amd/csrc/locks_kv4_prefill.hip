@@ -11,14 +11,20 @@
 // registers two tiles ahead, and writes their rows to LDS, K a tile before V.
 //
 // Matrix products and softmax are about as long as each other, and a wave that does
-// them in turn leaves both units half idle.  So they are skewed by a tile: the products
-// K(n + 1) Q^T stand between the exponentials of tile n, and V(n) P(n) between the
-// maximum of tile n + 1 and the conversion of the tiles behind it, issued alternately.
-// 8192 tokens, 32 / 8 heads, d 128, causal: 507 us, 1088 TFLOP/s (the three in turn, with
-// the tiles of locks_window.hip: 555); d 256 620 (1079), d 64 with 64 heads 650 (622).  Two
-// workgroups a CU at d 64 and 128, one at d 256 (registers).  What bounds it: matrix cores,
-// softmax and LDS about equally; a timing copy without the exponentials took 6 % less,
-// without LDS reads 7, without conversion and writes 13.
+// them in turn leaves both units half idle.  So at d 128 and 256 they are skewed by a tile:
+// the products K(n + 1) Q^T stand between the exponentials of tile n, and V(n) P(n) between
+// the maximum of tile n + 1 and the conversion of the tiles behind it, issued alternately.
+// 8192 tokens, 32 / 8 heads, d 128, causal: 500 to 520 us, 1060 to 1100 TFLOP/s (in turn,
+// with the tiles of locks_window.hip, 555); d 256, 16 / 4 heads, 620 to 630 us (in turn
+// 1080).  Two workgroups a CU at d 128, one at d 256 (registers).
+// At d 64 a tile has half of the products of d 128 for the same softmax, too few to stand
+// between it, and the skew's 215 registers leave a CU two workgroups, where in turn it holds
+// three, whose products and softmax overlap.  8192 tokens, 64 / 8 heads: skewed 648 us, in
+// turn 603 (with the tiles of locks_window.hip 620); 512 tokens on 16384 keys 98.3 and 96.6,
+// ragged window 68.9 and 68.3, 300 tokens 10.4 and 10.5.
+// What bounds it at d 128: matrix cores, softmax and LDS about equally; a timing copy
+// without the exponentials took 6 % less, without LDS reads 7, without conversion and
+// writes 13.
 #include "locks_attn.h"
 #include "locks_common.h"
 #include "locks_hip.h"
@@ -34,6 +40,10 @@ constexpr int P4_WAVES = 4;
 constexpr int P4_BLK = P4_WAVES * kWave;
 constexpr int P4_KT = 64;                   // keys per tile, 16 of them a wave's to convert
 static_assert(AT_ROWS == 32 * P4_WAVES && P4_KT == 16 * P4_WAVES, "rows and keys of a workgroup");
+// Whether a tile's products and softmax are skewed, and the workgroups that a CU has
+// registers for.
+constexpr bool p4_skewed(int head_dim) { return head_dim != 64; }
+constexpr int p4_resident(int head_dim) { return head_dim == 256 ? 1 : p4_skewed(head_dim) ? 2 : 3; }
 
 template <int D>
 struct P4Geom {
@@ -59,7 +69,7 @@ struct Kv4PrefillArgs {
 
 // PART: partials instead of the output.
 template <int D, bool PART>
-__global__ __launch_bounds__(P4_BLK, D == 256 ? 1 : 2) void kv4_prefill_kernel(const Kv4PrefillArgs a)
+__global__ __launch_bounds__(P4_BLK, p4_resident(D)) void kv4_prefill_kernel(const Kv4PrefillArgs a)
 {
     using GM = P4Geom<D>;
     constexpr int KT = P4_KT, ROWB = GM::ROWB, ND = D / 32;
@@ -378,8 +388,46 @@ __global__ __launch_bounds__(P4_BLK, D == 256 ? 1 : 2) void kv4_prefill_kernel(c
         for (int i = 0; i < NM; ++i) value(v_frag(vbuf(use), i), pf, i);
     };
 
+    // In turn: K(n) and V(n) are written, the codes of both of n + 1 on hand or on their way.
+    auto write_rows = [&](int n, auto buf) __attribute__((always_inline)) {
+        clear_nan(n, cv, buf());
+#pragma unroll
+        for (int x = 0; x < KI; ++x) write_k(kbuf(buf), ck, x);
+#pragma unroll
+        for (int x = 0; x < VI; ++x) write_v(vbuf(buf), cv, x);
+    };
+    auto in_turn = [&](int n, auto use, auto fill) __attribute__((always_inline)) {
+        lds_barrier();
+        if (n + 1 < n1) {
+            write_rows(n + 1, fill);
+            load_codes(n + 2, n + 2);
+        }
+        note_nan(n, use());
+        v16f s[2];
+#pragma unroll
+        for (int i = 0; i < NM; ++i) score(k_frag(kbuf(use), i), i, s);
+        settle(n, s, maximum(s));
+        const float mc = m == -INFINITY ? 0.f : m * a.scale_log2;
+        v8bf pf[KT / 16];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) weight(s, pf, e, mc);
+#pragma unroll
+        for (int i = 0; i < NM; ++i) value(v_frag(vbuf(use), i), pf, i);
+    };
+
     using I0 = std::integral_constant<int, 0>; using I1 = std::integral_constant<int, 1>;
-    if (n0 < n1) {
+    if constexpr (!p4_skewed(D)) {
+        if (n0 < n1) {
+            fetch(n0);
+            load_codes(n0, n0);
+            write_rows(n0, I0{});
+            load_codes(n0 + 1, n0 + 1);
+            for (int n = n0; n < n1; n += 2) {
+                in_turn(n, I0{}, I1{});
+                if (n + 1 < n1) in_turn(n + 1, I1{}, I0{});
+            }
+        }
+    } else if (n0 < n1) {
         v16f s0[2], s1[2];
         fetch(n0);
         load_codes(n0, n0);

@@ -133,3 +133,15 @@ def test_the_same_call_twice(d, G):
         one = call(x)
         for _ in range(3):
             assert all(torch.equal(a, b) for a, b in zip(call(x), one))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [1, 64, 65])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_prompts_of_each_count_of_tiles(d, n):
+    """One tile of keys to six, odd and even counts, for a tile of rows that sees them all or
+    some; more rows than one workgroup's."""
+    lens = [n + 64 * k for k in range(6)]
+    c = case(lens, [min(m, 70) for m in lens], 3, 4, d, 16, seed=n)
+    for window, sinks in ((0, 0), (65, 0), (64, 65)):
+        _agree(*_prefill(c, window, sinks), _exact(c, window, sinks))
