@@ -180,20 +180,24 @@ class LocksEngine:
     @torch.no_grad()
     def forward_dense(self, q, kv_cache, block_table, seq_lens, n_req: int, scale: float, out, *,
                       query_start_loc=None, n_decode: int = None, n_tokens: int = None, window: int = 0, sinks: int = 0,
-                      lse=None) -> None:
+                      lse=None, max_seq_len: int = 0) -> None:
         """One layer of any step with attention over the whole row, or over the
         last ``window`` tokens and the first ``sinks``, read from the paged cache (in
         bf16 or in 4 bits).
         The first ``n_decode`` requests have one new token each, in rows 0 to
         ``n_decode`` - 1 (default: all, without ``query_start_loc``; none with it),
         the others the rows that ``query_start_loc`` gives.  Padding takes no
-        token: it stands behind the requests with one, or after ``n_decode``."""
+        token: it stands behind the requests with one, or after ``n_decode``.
+        ``max_seq_len``: an upper bound of the lengths, where the caller's host knows
+        one; else the calls size themselves for the table, ``max_model_len`` tokens,
+        and short requests take longer (a length past the bound is attended to all
+        the same)."""
         if n_decode is None:
             n_decode = n_req if query_start_loc is None else 0
         if not 0 <= n_decode <= n_req or (n_decode < n_req and query_start_loc is None):
             raise ValueError(f"n_decode {n_decode} of {n_req} requests"
                              + ("" if query_start_loc is not None else " and no query_start_loc"))
-        kw = dict(scale=scale, window=window, sinks=sinks, lse=lse)
+        kw = dict(scale=scale, window=window, sinks=sinks, lse=lse, max_seq_len=max_seq_len)
         if n_decode:
             window_decode(q, kv_cache, block_table, seq_lens, out, self._ws(), n_req=n_decode, **kw)
         if n_decode < n_req:

@@ -145,3 +145,52 @@ def test_prompts_of_each_count_of_tiles(d, n):
     c = case(lens, [min(m, 70) for m in lens], 3, 4, d, 16, seed=n)
     for window, sinks in ((0, 0), (65, 0), (64, 65)):
         _agree(*_prefill(c, window, sinks), _exact(c, window, sinks))
+
+
+def test_engine_passes_the_bound_of_lengths(monkeypatch):
+    """Both calls of a mixed step get the caller's bound (the table's width sizes them else)."""
+    from locks.backend import engine
+    got = []
+    for name in ("window_decode", "window_prefill"):
+        monkeypatch.setattr(engine, name, lambda *a, name=name, **kw: got.append((name, kw["max_seq_len"])))
+    eng = engine.LocksEngine.__new__(engine.LocksEngine)
+    eng._dense_ws = object()
+    rows = torch.zeros(4, 8, dtype=torch.int32)
+    for bound in (0, 500):
+        eng.forward_dense(None, None, rows, rows[:, 0], 4, 1.0, None, query_start_loc=rows[0], n_decode=2,
+                          **({"max_seq_len": bound} if bound else {}))
+    assert got == [("window_decode", 0), ("window_prefill", 0), ("window_decode", 500), ("window_prefill", 500)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("four", [False, True])
+def test_engine_with_a_wide_table(four):
+    """Short requests in an engine for long ones: the same rows with a bound of the lengths
+    (exact, generous or too low) and without."""
+    from locks import LocksConfig
+    from locks.backend.engine import LocksEngine
+    n_kv, G, d, page, blocks = 2, 4, 128, 16, 80
+    selected = torch.zeros(blocks, 2, page, n_kv, d, dtype=torch.bfloat16, device="cuda")
+    eng = LocksEngine(LocksConfig(budget_pages=8), [selected], num_heads_q=n_kv * G, num_heads_kv=n_kv, head_dim=d,
+                      block_size=page, max_num_seqs=4, max_model_len=131072, max_num_batched_tokens=1024)
+    cache, t = eng.kv4_cache() if four else selected, eng.block_tables()
+    lens, new = [500, 281, 64], [500, 281, 64]
+    for n_decode in (0, 3):
+        T = sum(new)
+        x = inputs(T, n_kv * G, n_kv, d, d, 1, seed=n_decode)
+        t.step(torch.arange(3, dtype=torch.int32, device="cuda"), torch.tensor(new, dtype=torch.int32, device="cuda"),
+               n_req=3, n_tokens=T)
+        assert t.block_table.shape[1] == 8192
+        eng.write_qkv(0, x["q"], x["k"], x["v"], x["pos"][0].contiguous(), t.slot_mapping[:T], None, torch.zeros_like(x["q"]),
+                      kv_cache=cache)
+        at = [torch.arange(n, device="cuda") for n in lens]
+        slots = [t.block_table[r].long()[a // page] * page + a % page for r, a in enumerate(at)]
+        kv = [_read(cache, s) if four else (cache[s // page, 0, s % page], cache[s // page, 1, s % page]) for s in slots]
+        c = dict(q=x["q"], k=[k for k, _ in kv], v=[v for _, v in kv], lens=lens, new=new, n_kv=n_kv, G=G, d=d, scale=0.09)
+        want = _exact(c, 0, 0)
+        for bound in (0, max(lens), 4000, 16):
+            out, lse = torch.zeros_like(x["q"]), torch.zeros(T, n_kv * G, device="cuda")
+            eng.forward_dense(x["q"], cache, t.block_table, t.seq_lens, 3, 0.09, out, query_start_loc=t.query_start_loc,
+                              n_decode=n_decode, lse=lse, max_seq_len=bound)
+            _agree(out, lse, want)
+        lens, new = [n + 1 for n in lens], [1, 1, 1]
