@@ -66,7 +66,13 @@ inline long bound_keys(int32_t max_seq_len, int32_t bt_cols, int32_t page) {
     const long cap = (long)bt_cols * page;
     return max_seq_len > 0 && max_seq_len < cap ? max_seq_len : cap;
 }
-
+// Splits of a row's keys in a call of many tokens: one once there are 256 workgroups, else
+// about 512 workgroups of at least 4 tiles of key_tile keys.
+inline int prefill_splits(long tiles, int n_kv, long max_keys, int key_tile) {
+    const long wgs = tiles * n_kv;
+    if (wgs >= 256) return 1;
+    return clampi((512 + wgs - 1) / wgs, 1, clampi(max_keys / (4 * key_tile), 1, 64));
+}
 
 // Bytes of a call's partials, and where they stand in its workspace.
 inline int64_t part_bytes(int64_t rows, int splits, int D) { return rows * splits * (D + 2) * 4; }
@@ -88,7 +94,6 @@ int32_t check_kv4(const char* what, const void* cache, int64_t sb, int64_t sh, i
 
 // Workspace of a single-token call on one (locks_kv4.hip).
 int64_t kv4_workspace(int n_req, int n_kv, int G, int head_dim);
-// Splits of a row's keys in a call of many tokens on one.
-int kv4_prefill_splits(long tiles, int n_kv, long max_keys, int head_dim);
+constexpr int P4_KT = 64;                   // keys per tile of a call of many tokens on one
 
 }  // namespace locks

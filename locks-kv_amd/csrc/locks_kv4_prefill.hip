@@ -38,7 +38,7 @@ namespace locks {
 
 constexpr int P4_WAVES = 4;
 constexpr int P4_BLK = P4_WAVES * kWave;
-constexpr int P4_KT = 64;                   // keys per tile, 16 of them a wave's to convert
+// (16 keys of a tile are a wave's to convert)
 static_assert(AT_ROWS == 32 * P4_WAVES && P4_KT == 16 * P4_WAVES, "rows and keys of a workgroup");
 // Whether a tile's products and softmax are skewed, and the workgroups that a CU has
 // registers for.
@@ -496,14 +496,6 @@ __global__ __launch_bounds__(P4_BLK, p4_resident(D)) void kv4_prefill_kernel(con
     }
 }
 
-// One split once there are 256 workgroups, else about 512 of at least 4 key tiles (the
-// rule of the bf16 cache's calls: 512 tokens of 32 heads on 65536 keys, 4 splits).
-int kv4_prefill_splits(long tiles, int n_kv, long max_keys, int head_dim) {
-    const long wgs = tiles * n_kv;
-    if (wgs >= 256) return 1;
-    return clampi((512 + wgs - 1) / wgs, 1, clampi(max_keys / (4 * P4_KT), 1, 64));
-}
-
 }  // namespace locks
 
 using namespace locks;
@@ -531,7 +523,7 @@ extern "C" int32_t locks_kv4_prefill(
     if (n_req == 0 || n_tokens == 0) return 0;
     const long bound = bound_keys(max_seq_len, bt_cols, page), reach = (long)window + sinks + n_tokens;
     const long tiles = prefill_tiles(n_tokens, n_req, G);
-    const int ns = kv4_prefill_splits(tiles, n_kv, window && reach < bound ? reach : bound, head_dim);
+    const int ns = prefill_splits(tiles, n_kv, window && reach < bound ? reach : bound, P4_KT);
     const int64_t rows = (int64_t)n_tokens * n_kv * G;
     LOCKS_REQUIRE(tiles * n_kv * ns <= 0x7fffffffL, "%s: too many tokens and heads for one launch", what);
     Kv4PrefillArgs a{q, q_stride_tok, q_stride_head, cache, c_stride_block, c_stride_head, block_table, bt_stride, seq_lens,

@@ -47,9 +47,11 @@ typedef unsigned short v2us __attribute__((ext_vector_type(2)));
 constexpr int AT_WAVES = 4;
 constexpr int AT_BLK = AT_WAVES * kWave;
 
+constexpr int at_key_tile(int head_dim) { return head_dim == 256 ? 32 : 64; }    // keys per tile
+
 template <int D>
 struct AtGeom {
-    static constexpr int KT = D == 256 ? 32 : 64;        // keys per tile
+    static constexpr int KT = at_key_tile(D);
     static constexpr int NST = D == 128 ? 2 : 3;        // tiles in LDS: one in use, the others on the way
     static constexpr int ROWB = 2 * D;                  // bytes of a K or V row
     static constexpr int TILEB = KT * ROWB;
@@ -627,17 +629,10 @@ static int decode_splits(int n_req, int n_kv, long max_keys, bool even) {
     const long most = !even ? 1 : (steps + 63) / 64 < cap ? (steps + 63) / 64 : cap;
     return clampi(fill > most ? fill : most, 1, clampi((steps + 7) / 8, 1, 64));
 }
-// Many tokens: one split once there are 256 workgroups, else about 512 of at
-// least 4 key tiles.
-static int prefill_splits(long tiles, int n_kv, long max_keys, int head_dim) {
-    const long wgs = tiles * n_kv, kt = head_dim == 256 ? 32 : 64;
-    if (wgs >= 256) return 1;
-    return clampi((512 + wgs - 1) / wgs, 1, clampi(max_keys / (4 * kt), 1, 64));
-}
 // A prefix: one workgroup per CU, the other place on it is for the own keys (64
 // requests on 32K tokens: 16 splits 82 us, 32 88, 8 106).
 static int shared_splits(long tiles, int n_kv, long max_keys, int head_dim) {
-    const long wgs = tiles * n_kv, kt = head_dim == 256 ? 32 : 64;
+    const long wgs = tiles * n_kv, kt = at_key_tile(head_dim);
     return clampi((256 + wgs - 1) / wgs, 1, clampi(max_keys / (4 * kt), 1, 64));
 }
 
@@ -706,16 +701,13 @@ extern "C" int64_t locks_attn_workspace_bytes(int32_t max_reqs, int32_t max_toke
         most = b > most ? b : most;
     }
     for (int n = 1; n <= max_tokens && prefill_tiles(n, 1, G) * n_kv < 256; ++n) {
-        const int64_t b = part_bytes((int64_t)n * n_kv * G, prefill_splits(prefill_tiles(n, 1, G), n_kv, long_row, head_dim), head_dim);
+        // (the smaller tile of keys: that of bf16, or the same)
+        static_assert(at_key_tile(64) <= P4_KT && at_key_tile(128) <= P4_KT && at_key_tile(256) <= P4_KT, "splits of a row");
+        const int64_t b = part_bytes((int64_t)n * n_kv * G, prefill_splits(prefill_tiles(n, 1, G), n_kv, long_row, at_key_tile(head_dim)), head_dim);
         most = b > most ? b : most;
     }
-    // the same calls on a cache in 4 bits
-    if (max_reqs > 0) {
+    if (max_reqs > 0) {                     // single-token calls on a cache in 4 bits
         const int64_t b = kv4_workspace(max_reqs < 65535 ? max_reqs : 65535, n_kv, G, head_dim);
-        most = b > most ? b : most;
-    }
-    for (int n = 1; n <= max_tokens && prefill_tiles(n, 1, G) * n_kv < 256; ++n) {
-        const int64_t b = part_bytes((int64_t)n * n_kv * G, kv4_prefill_splits(prefill_tiles(n, 1, G), n_kv, long_row, head_dim), head_dim);
         most = b > most ? b : most;
     }
     return most;
@@ -779,7 +771,7 @@ extern "C" int32_t locks_window_prefill(
     if (n_req == 0 || n_tokens == 0) return 0;
     const long keys = window ? (long)window + sinks + n_tokens : bound_keys(max_seq_len, bt_cols, page);
     const long tiles = prefill_tiles(n_tokens, n_req, G);
-    int ns = prefill_splits(tiles, n_kv, keys < bound_keys(max_seq_len, bt_cols, page) ? keys : bound_keys(max_seq_len, bt_cols, page), head_dim);
+    int ns = prefill_splits(tiles, n_kv, keys < bound_keys(max_seq_len, bt_cols, page) ? keys : bound_keys(max_seq_len, bt_cols, page), at_key_tile(head_dim));
     const int64_t rows = (int64_t)n_tokens * n_kv * G;
     LOCKS_REQUIRE(tiles * n_kv * ns <= 0x7fffffffL, "%s: too many tokens and heads for one launch", what);
     Partials p{};
