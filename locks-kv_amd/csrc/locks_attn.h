@@ -29,8 +29,9 @@ __device__ __forceinline__ int group_pages(const int* __restrict__ gstart, const
 }
 
 // Partials of a call: per (token or request, kv head) row, split and query head
-// of the group, m (the maximum, as a natural-log score) and l (the sum) and acc
-// (D) in fp32.  A split without keys leaves m = -inf, l = 0 and no acc.
+// of the group, m (the maximum, as a natural-log score; base 2 where the cache has 4 bits),
+// l (the sum) and acc
+// (D) in fp32.  A split without keys leaves m = -inf and l = 0, and no acc that counts.
 struct Partials {
     float* m; float* l; float* acc;
     int splits;                             // of a row

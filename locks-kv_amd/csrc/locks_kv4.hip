@@ -20,12 +20,13 @@
 // one row and a start of another, whose partials go to its two slots.
 //
 // Bound by memory: 17 d bytes for K and V of 16 keys and a head, read once, past the
-// caches.  1M keys of 8 heads, d 128: 180 us, 6.4 TB/s; 131072 keys 33 us (28 and the
+// caches.  1M keys of 8 heads, d 128: 180 us, 6.3 TB/s; 131072 keys 33 us (28 and the
 // merge: the chain of lengths, block ids and first tiles, and the join, are 10 of them); 32
 // requests of 1 to 32768 keys 54 us, 5.3 TB/s.  Two workgroups a CU, two steps on their
 // way: 70 KB a CU, more than latency x rate needs (three and four steps, and three
-// workgroups, were slower).  At d 64 the instructions of a step bound it: 1M keys 111 us,
-// 5.1 TB/s.
+// workgroups, were slower).  At d 64 a step has 0.7 of d 128's vector instructions for half
+// of the bytes: 1M keys 111 us, 5.1 TB/s, the vector units busy 55 % of the time (d 128 48,
+// d 256 38) and waves waiting for half of theirs.
 #include "locks_attn.h"
 #include "locks_common.h"
 #include "locks_hip.h"
@@ -45,10 +46,12 @@ constexpr int K4_SHARE = 24;                // tiles that a share has at least
 // Workgroups that a CU has registers for: at d 64 128 of them do (300 requests of 1500 keys
 // 56.1 us with three workgroups a CU, 51.3 with four).
 constexpr int kv4_resident(int head_dim) { return head_dim == 64 ? 4 : 2; }
-// Shares at most: two workgroups a CU, or three at d 64, where the instructions of a step
-// bound it (1M keys of 8 heads 122 -> 111 us, 64 requests of 4096 41.0 -> 37.5, 16 of 3000
-// 12.6 -> 13.0; four 110, 37.1 and 13.0).  Three cost more than they give at d 128 (131072
-// keys 33.2 -> 37.9 us) and where a group's partials are large (16 heads 19.7 -> 21.0).
+// Shares at most: two workgroups a CU, or three at d 64, whose waves have more to issue for
+// their bytes (1M keys of 8 heads 122 -> 111 us, 64 requests of 4096 41.0 -> 37.5, of 1500
+// 23.3 -> 21.9; four 110 and 37.1).  Calls between cost up to 3 % by it: with 4 heads 16
+// requests of 3000 keys 13.0 -> 13.3, 32 of 2000 14.5 -> 14.9, 131072 keys 18.2 -> 18.7.
+// Three cost more than they give at d 128 (131072 keys 33.2 -> 37.9 us) and where a group's
+// partials are large (16 heads 19.7 -> 21.0).
 static int kv4_grid(int head_dim, int G) { return head_dim == 64 && G <= 8 ? 768 : 512; }
 constexpr float kLn2 = 0.69314718055994530942f;
 
@@ -107,7 +110,7 @@ __device__ __forceinline__ double wave_incl_scan(double v) {
     return v;
 }
 
-// Bits 2 lo .. of two words as one: {low or high halves of a, of b}.
+// The low (high) halves of two words as one, a's below b's.
 __device__ __forceinline__ uint32_t lows(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x05040100u); }
 __device__ __forceinline__ uint32_t highs(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
 

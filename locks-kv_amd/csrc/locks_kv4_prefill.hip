@@ -14,17 +14,20 @@
 // them in turn leaves both units half idle.  So at d 128 and 256 they are skewed by a tile:
 // the products K(n + 1) Q^T stand between the exponentials of tile n, and V(n) P(n) between
 // the maximum of tile n + 1 and the conversion of the tiles behind it, issued alternately.
-// 8192 tokens, 32 / 8 heads, d 128, causal: 500 to 520 us, 1060 to 1100 TFLOP/s (in turn,
-// with the tiles of locks_window.hip, 555); d 256, 16 / 4 heads, 620 to 630 us (in turn
-// 1080).  Two workgroups a CU at d 128, one at d 256 (registers).
+// 8192 tokens, 32 / 8 heads, d 128, causal: 500 to 533 us, 1030 to 1100 TFLOP/s (in turn,
+// with the tiles of locks_window.hip, 555), by the card: its clock falls to 1.8 GHz under
+// the call; d 256, 16 / 4 heads, 620 to 630 us (in turn 1080).  Two workgroups a CU at d
+// 128, one at d 256 (registers).
 // At d 64 a tile has half of the products of d 128 for the same softmax, too few to stand
 // between it, and the skew's 215 registers leave a CU two workgroups, where in turn it holds
 // three, whose products and softmax overlap.  8192 tokens, 64 / 8 heads: skewed 648 us, in
 // turn 603 (with the tiles of locks_window.hip 620); 512 tokens on 16384 keys 98.3 and 96.6,
 // ragged window 68.9 and 68.3, 300 tokens 10.4 and 10.5.
-// What bounds it at d 128: matrix cores, softmax and LDS about equally; a timing copy
-// without the exponentials took 6 % less, without LDS reads 7, without conversion and
-// writes 13.
+// What bounds it, by counters: at d 128 LDS (busy 72 % of the time), the vector units (55)
+// and the matrix cores (49) together, and a timing copy without the exponentials took 6 %
+// less, without LDS reads 7, without conversion and writes 13; at d 64 the vector units
+// (76; LDS 63, matrix cores 40); at d 256 the one wave a SIMD, which waits 31 % of its time
+// (LDS 49, vector units 35, matrix cores 35).
 #include "locks_attn.h"
 #include "locks_common.h"
 #include "locks_hip.h"

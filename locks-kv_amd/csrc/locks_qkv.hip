@@ -492,7 +492,8 @@ __global__ __launch_bounds__(QK_BLK) void qkv_staged_kernel(const QkvArgs a)
                     }
                     f = 1.0 / sqrt(head_sum<D>(sum) * (1.0 / D) + (double)a.eps);
                 }
-                // entry x weight x angle is exact: the norm's factor comes last
+                // the norm's factor comes last: entry x weight x angle is exact with bf16
+                // weights (40 bits), and within 2^-53 of itself with fp32 ones (56)
                 auto values = [&](int h) __attribute__((always_inline)) {
                     four(raw[i], h, z);
                     if (normed) times(z, w_s[1] + e0 + 4 * h);
